@@ -249,6 +249,84 @@ int b200dq_gemm_static_scratch(const b200dq_gemm_args* args, void* cuda_stream);
 int b200dq_static_scratch_check(const b200dq_gemm_args* args, int32_t sm_count, size_t* needed_bytes,
                                 size_t* capacity_bytes);
 
+/* ---- 8-bit floating point with a scale for each block of 128 ---------------------------
+ * Values are code * scale, codes e4m3 or e5m2 bytes, scales fp32: one per row and 128 columns for
+ * activations and gradients, one per 128 x 128 block for weights. */
+enum b200dq_fp8_type { B200DQ_FP8_E4M3 = 0, B200DQ_FP8_E5M2 = 1 };
+enum b200dq_float_type { B200DQ_F16 = 0, B200DQ_BF16 = 1, B200DQ_F32 = 2 };
+enum b200dq_fp8_quant_mode {
+  B200DQ_FP8_OF_ROWS = 0,          /* x (rows, cols)                                              */
+  B200DQ_FP8_OF_SILU_MUL = 1,      /* silu(g) * u of x = [g | u], (rows, 2 cols)                   */
+  B200DQ_FP8_OF_SILU_MUL_GRAD = 2  /* [dg | du], (rows, 2 cols), from x = [g | u] and d (rows, cols) */
+};
+
+/* scale = max |v| of the block / largest finite code (448, 57344), at least 2^-126;
+ * code = rn(v * (1 / scale)), ties to even, all in fp32. A block that holds NaN or an infinity gets
+ * that as its scale. codes: rows of ld_codes bytes; scales (rows, ceil(columns of the result / 128)),
+ * contiguous. ld_x, ld_d: row pitches in elements. Rows and pitches that are multiples of 16 columns on
+ * 16-byte boundaries take the fast kernel, everything else a slower one with the same results. */
+int b200dq_quant_fp8(int32_t mode, const void* x, int64_t ld_x, const void* d, int64_t ld_d, void* codes,
+                     int64_t ld_codes, float* scales, int64_t rows, int32_t cols, int32_t in_type, int32_t fp8_type,
+                     void* cuda_stream);
+
+/* The same over 128 x 128 blocks of `batch` contiguous (N, K) matrices: codes (batch, N, ld_codes),
+ * scales (batch, ceil(N / 128), ceil(K / 128)). */
+int b200dq_quant_fp8_blocks(const void* x, void* codes, int64_t ld_codes, float* scales, int64_t batch, int32_t N,
+                            int32_t K, int32_t in_type, int32_t fp8_type, void* cuda_stream);
+
+/* Arguments of b200dq_gemm_fp8: C = A * W^T with A (M, K) and W (N, K), C (M, N); or with trans_w
+ * C = A * W with A (M, N), C (M, K): the gradient of the input, from the same weight bytes. */
+typedef struct b200dq_fp8_gemm_args {
+  const void* a;            /* codes, rows of lda bytes                                       */
+  const float* a_scale;     /* (M, ceil(contraction / 128)), row pitch ld_a_scale elements    */
+  const void* w;            /* codes, (num_groups or 1) matrices of N rows of ldw bytes       */
+  const float* w_scale;     /* (num_groups or 1, ceil(N / 128), ceil(K / 128)), contiguous    */
+  void* c;                  /* output, row-major contiguous                                   */
+  const void* counts;       /* grouped: rows of each group, num_groups values in device memory */
+  int64_t lda, ld_a_scale, ldw;
+  int64_t w_group_stride;   /* bytes between the matrices of consecutive groups               */
+  int32_t M, N, K;
+  int32_t num_groups;       /* 0: one product; else rows of A and C are sorted by group        */
+  int32_t counts_int64;
+  int32_t a_type, w_type;   /* enum b200dq_fp8_type, any pairing                              */
+  int32_t out_type;         /* f16, bf16 or f32                                               */
+  int32_t trans_w;
+  int32_t token_tile;       /* 0: chosen; 16, 32, 64: tokens are the tile's columns, 128: its lanes */
+  int32_t split;            /* 0: chosen; else CTAs (1 to 8) that share a tile's contraction  */
+} b200dq_fp8_gemm_args;
+
+/* Sums are fp32: exact products added on the tensor cores within a block of 128, blocks scaled and
+ * added in fp32 registers; one rounding to the output type. a, w, c and both pitches are multiples of
+ * 16 bytes (c: of its element size). Deterministic; no scratch. Grouped: counts that do not sum to M
+ * are clamped to the rows that exist, and rows of C behind the last group are not written. */
+int b200dq_gemm_fp8(const b200dq_fp8_gemm_args* args, void* cuda_stream);
+
+/* ---- token exchange of a mixture-of-experts layer ---------------------------------------
+ * experts (tokens, top_k), int32 or int64: row_of[t, s] = rows of smaller experts + earlier pairs (in
+ * (token, slot) order) of the same expert; counts (num_experts) = rows of each expert. The token rows
+ * x (tokens, width) go to out[row_of[t, s]]: copied, or with `scales` quantised as by
+ * b200dq_quant_fp8 to fp8_type (out: rows of ld_out bytes). A pair whose id is outside
+ * [0, num_experts) sorts behind the last expert: its row is zeros and row_of = -1 - row. scratch:
+ * b200dq_exchange_scratch_bytes() bytes (may be 0). num_experts <= 1024. The reference's layer does
+ * this with argsort, bincount and gathers (examples/fusedmoe/example_fusedmoe_torch.py:65-91). */
+size_t b200dq_exchange_scratch_bytes(int64_t tokens, int32_t top_k, int32_t num_experts);
+int b200dq_exchange_dispatch(const void* experts, int32_t experts_int64, int64_t tokens, int32_t top_k,
+                             int32_t num_experts, const void* x, int64_t ld_x, int32_t width, int32_t type, void* out,
+                             int64_t ld_out, float* scales, int32_t fp8_type, int64_t* row_of, int64_t* counts,
+                             void* scratch, size_t scratch_bytes, void* cuda_stream);
+
+/* out[t] = sum over s of weights[t, s] * y[row_of[t, s]] (weights NULL: all one; negative row_of: no
+ * term), fp32 sums in slot order, one rounding. Also the gradient of the copying dispatch. */
+int b200dq_exchange_sum(const void* y, const int64_t* row_of, const float* weights, void* out, int64_t tokens,
+                        int32_t top_k, int32_t width, int32_t type, void* cuda_stream);
+
+/* Gradient of the weighted sum: d_y[row_of[t, s]] = weights[t, s] * d_out[t] (zeros for rows behind the
+ * last expert), d_weights[t, s] = <d_out[t], y[row_of[t, s]]> in fp32. Either output may be NULL, y
+ * too when d_weights is. */
+int b200dq_exchange_sum_grad(const void* d_out, const void* y, const int64_t* row_of, const float* weights, void* d_y,
+                             float* d_weights, int64_t tokens, int32_t top_k, int32_t width, int32_t type,
+                             void* cuda_stream);
+
 /* Reads the device status word of the current device (synchronises `stream`).
  * Returns 0 if no kernel recorded an error since the last reset, else -1 with a
  * message naming the wait that gave up; resets the word. */

@@ -18,6 +18,9 @@ LIB_PATH = os.path.join(_HERE, "libb200dq.so")
 WF_U4_SZ, WF_U4_RAW, WF_S4_RAW, WF_FP4_E8M0, WF_I2_I8, WF_I4_I8, WF_U2_SZ, WF_LUT4_S = range(8)
 ACT_F16, ACT_BF16, ACT_I8 = range(3)
 OUT_F16, OUT_BF16, OUT_F32, OUT_I32 = range(4)
+FP8_E4M3, FP8_E5M2 = range(2)
+F16, BF16, F32 = range(3)
+FP8_OF_ROWS, FP8_OF_SILU_MUL, FP8_OF_SILU_MUL_GRAD = range(3)
 GF_TRANS_C, GF_HAS_BIAS, GF_ROW_SCALE, GF_FP4_SIMPLE = 1, 2, 4, 16
 
 EXPORTED_SYMBOLS = (
@@ -40,6 +43,13 @@ EXPORTED_SYMBOLS = (
     "b200dq_silu_mul",
     "b200dq_unpack_int4_to_int8",
     "b200dq_moe_combine",
+    "b200dq_quant_fp8",
+    "b200dq_quant_fp8_blocks",
+    "b200dq_gemm_fp8",
+    "b200dq_exchange_scratch_bytes",
+    "b200dq_exchange_dispatch",
+    "b200dq_exchange_sum",
+    "b200dq_exchange_sum_grad",
 )
 
 
@@ -78,6 +88,34 @@ class GemmArgs(ctypes.Structure):
         ("c_peers", ctypes.c_void_p * 7),
         ("num_peers", ctypes.c_int32),
         ("code_table", ctypes.c_float * 16),
+    ]
+
+
+class Fp8GemmArgs(ctypes.Structure):
+    """``struct b200dq_fp8_gemm_args``."""
+
+    _fields_ = [
+        ("a", ctypes.c_void_p),
+        ("a_scale", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("w_scale", ctypes.c_void_p),
+        ("c", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("lda", ctypes.c_int64),
+        ("ld_a_scale", ctypes.c_int64),
+        ("ldw", ctypes.c_int64),
+        ("w_group_stride", ctypes.c_int64),
+        ("M", ctypes.c_int32),
+        ("N", ctypes.c_int32),
+        ("K", ctypes.c_int32),
+        ("num_groups", ctypes.c_int32),
+        ("counts_int64", ctypes.c_int32),
+        ("a_type", ctypes.c_int32),
+        ("w_type", ctypes.c_int32),
+        ("out_type", ctypes.c_int32),
+        ("trans_w", ctypes.c_int32),
+        ("token_tile", ctypes.c_int32),
+        ("split", ctypes.c_int32),
     ]
 
 
@@ -127,6 +165,21 @@ def _declare(lib):
     lib.b200dq_unpack_int4_to_int8.argtypes = [vp, vp, ctypes.c_int64, vp]
     lib.b200dq_moe_combine.restype = ctypes.c_int
     lib.b200dq_moe_combine.argtypes = [vp, vp, vp, vp, ctypes.c_int64, i32, i32, i32, vp]
+    i64 = ctypes.c_int64
+    lib.b200dq_quant_fp8.restype = ctypes.c_int
+    lib.b200dq_quant_fp8.argtypes = [i32, vp, i64, vp, i64, vp, i64, vp, i64, i32, i32, i32, vp]
+    lib.b200dq_quant_fp8_blocks.restype = ctypes.c_int
+    lib.b200dq_quant_fp8_blocks.argtypes = [vp, vp, i64, vp, i64, i32, i32, i32, i32, vp]
+    lib.b200dq_gemm_fp8.restype = ctypes.c_int
+    lib.b200dq_gemm_fp8.argtypes = [ctypes.POINTER(Fp8GemmArgs), vp]
+    lib.b200dq_exchange_scratch_bytes.restype = sz
+    lib.b200dq_exchange_scratch_bytes.argtypes = [i64, i32, i32]
+    lib.b200dq_exchange_dispatch.restype = ctypes.c_int
+    lib.b200dq_exchange_dispatch.argtypes = [vp, i32, i64, i32, i32, vp, i64, i32, i32, vp, i64, vp, i32, vp, vp, vp, sz, vp]
+    lib.b200dq_exchange_sum.restype = ctypes.c_int
+    lib.b200dq_exchange_sum.argtypes = [vp, vp, vp, vp, i64, i32, i32, i32, vp]
+    lib.b200dq_exchange_sum_grad.restype = ctypes.c_int
+    lib.b200dq_exchange_sum_grad.argtypes = [vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, vp]
     lib.b200dq_check_status.restype = ctypes.c_int
     lib.b200dq_check_status.argtypes = [vp]
 

@@ -24,6 +24,9 @@
 #include "mxf4_launch.h"
 #include "peak_launch.h"
 #include "int8_skinny_launch.h"
+#include "exchange_launch.h"
+#include "fp8_launch.h"
+#include "fp8_quant_launch.h"
 
 namespace {
 
@@ -486,6 +489,113 @@ int run_gemm(const char* who, const b200dq_gemm_args* a, void* scratch, size_t s
   return fail("%s: no kernel for weight format %d with activation type %d", who, wf, act);
 }
 
+// ---- block-scaled fp8 products ---------------------------------------------------------------
+
+struct Fp8Plan {
+  int token_tile;        // 16, 32, 64: tokens in columns; 128: tokens on lanes
+  int split;
+  long long tiles;       // clusters to launch (an upper bound when the counts are on the device)
+};
+
+// Token tile and split of a product with `rows` rows (in `groups` groups, or 0), `p_tiles` tiles of 128
+// output columns and `q_blocks` blocks of contraction.
+//  - Tile: tokens in columns as long as a tile holds them all (a group's mean share, when grouped): the weights
+//    are then read once and the tensor cores' 128 lanes are full of them. From 65 tokens on they fill the
+//    lanes themselves, and a reading thread's scale is one number instead of a vector.
+//  - Split: as many CTAs as the GPU holds at once (two per SM below 128 tokens), at most 8 per tile (the
+//    portable cluster size), each with at least two blocks.
+Fp8Plan plan_fp8(int rows, int groups, int p_tiles, int q_blocks, int sms, int token_tile, int split) {
+  Fp8Plan plan;
+  const long long share = groups > 0 ? (rows + groups - 1) / groups : rows;
+  plan.token_tile = token_tile > 0 ? token_tile : share <= 16 ? 16 : share <= 32 ? 32 : share <= 64 ? 64 : 128;
+  long long token_tiles = (rows + plan.token_tile - 1) / plan.token_tile;
+  if (groups > 0) token_tiles = rows / plan.token_tile + std::min<long long>(groups, rows);
+  plan.tiles = token_tiles * p_tiles;
+  const long long slots = static_cast<long long>(sms) * (plan.token_tile >= 128 ? 1 : 2);
+  long long s = split > 0 ? split : slots / plan.tiles;
+  s = std::min<long long>(s, split > 0 ? q_blocks : q_blocks / 2);
+  plan.split = static_cast<int>(std::max<long long>(1, std::min<long long>(s, 8)));
+  return plan;
+}
+
+int encode_fp8_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                   cuuint32_t box_rows) {
+  cuuint32_t box[3] = {kFp8BoxBytes, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, static_cast<cuuint32_t>(rank), const_cast<void*>(base),
+                              dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail("gemm_fp8: cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(r));
+  return 0;
+}
+
+int check_fp8_gemm(const b200dq_fp8_gemm_args* a) {
+  if (a->a == nullptr || a->a_scale == nullptr || a->w == nullptr || a->w_scale == nullptr || a->c == nullptr)
+    return fail("gemm_fp8: null pointer");
+  if (a->M <= 0 || a->N <= 0 || a->K <= 0) return fail("gemm_fp8: M, N, K must be positive (got %d, %d, %d)", a->M, a->N, a->K);
+  if (a->num_groups < 0 || a->num_groups > 65535) return fail("gemm_fp8: num_groups=%d outside [0, 65535]", a->num_groups);
+  if (a->num_groups > 0 && a->counts == nullptr) return fail("gemm_fp8: a grouped call needs the counts");
+  const int inner = a->trans_w ? a->N : a->K;
+  if (a->lda < inner || a->lda % 16 != 0) return fail("gemm_fp8: rows of A must be a multiple of 16 bytes apart (lda=%lld for %d columns)", static_cast<long long>(a->lda), inner);
+  if (a->ldw < a->K || a->ldw % 16 != 0) return fail("gemm_fp8: rows of W must be a multiple of 16 bytes apart (ldw=%lld for %d columns)", static_cast<long long>(a->ldw), a->K);
+  if (a->num_groups > 1 && (a->w_group_stride < a->ldw * a->N || a->w_group_stride % 16 != 0))
+    return fail("gemm_fp8: the matrices of W must lie a multiple of 16 bytes apart and not overlap");
+  if (a->ld_a_scale < (inner + 127) / 128) return fail("gemm_fp8: ld_a_scale=%lld is less than the %d scales of a row", static_cast<long long>(a->ld_a_scale), (inner + 127) / 128);
+  if (a->a_type < 0 || a->a_type > FP8_E5M2 || a->w_type < 0 || a->w_type > FP8_E5M2) return fail("gemm_fp8: operands must be e4m3 or e5m2");
+  if (a->out_type != OUT_F16 && a->out_type != OUT_BF16 && a->out_type != OUT_F32) return fail("gemm_fp8: output must be f16, bf16 or f32");
+  if ((reinterpret_cast<uintptr_t>(a->a) & 15) != 0 || (reinterpret_cast<uintptr_t>(a->w) & 15) != 0)
+    return fail("gemm_fp8: a and w must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(a->a_scale) & 3) != 0 || (reinterpret_cast<uintptr_t>(a->w_scale) & 3) != 0 ||
+      (reinterpret_cast<uintptr_t>(a->c) & (out_elem_size(a->out_type) - 1)) != 0)
+    return fail("gemm_fp8: scales and output must be aligned to their elements");
+  if (a->token_tile != 0 && a->token_tile != 16 && a->token_tile != 32 && a->token_tile != 64 && a->token_tile != 128)
+    return fail("gemm_fp8: token_tile must be 0, 16, 32, 64 or 128 (got %d)", a->token_tile);
+  if (a->split < 0 || a->split > 8) return fail("gemm_fp8: split must be 0 to 8 (got %d)", a->split);
+  return 0;
+}
+
+int run_gemm_fp8(const b200dq_fp8_gemm_args* a, const DeviceState* ds, cudaStream_t stream) {
+  const int inner = a->trans_w ? a->N : a->K, outer = a->trans_w ? a->K : a->N;
+  const int n_blocks = (a->N + 127) / 128, k_blocks = (a->K + 127) / 128;
+  Fp8GemmParams p;
+  memset(&p, 0, sizeof(p));
+  p.a_scale = a->a_scale;
+  p.ld_a_scale = a->ld_a_scale;
+  p.w_scale = a->w_scale;
+  p.ws_p = a->trans_w ? 1 : k_blocks;
+  p.ws_q = a->trans_w ? k_blocks : 1;
+  p.ws_group = static_cast<long long>(n_blocks) * k_blocks;
+  p.c = a->c;
+  p.ldc = outer;
+  p.M = a->M; p.P = outer;
+  p.q_blocks = (inner + 127) / 128;
+  p.p_tiles = (outer + 127) / 128;
+  p.out_type = a->out_type;
+  p.a_fmt = a->a_type; p.w_fmt = a->w_type;
+  p.trans_w = a->trans_w ? 1 : 0;
+  p.c_vec = outer % 4 == 0 && (reinterpret_cast<uintptr_t>(a->c) & (4 * out_elem_size(a->out_type) - 1)) == 0;
+  p.counts = a->num_groups > 0 ? a->counts : nullptr;
+  p.counts_int64 = a->counts_int64;
+  p.num_groups = a->num_groups;
+  p.status = ds->status;
+  const Fp8Plan plan = plan_fp8(a->M, a->num_groups, p.p_tiles, p.q_blocks, ds->sm_count, a->token_tile, a->split);
+  p.split = plan.split;
+  CUtensorMap tmap_a, tmap_w;
+  const cuuint64_t a_dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(a->M)};
+  const cuuint64_t a_strides[1] = {static_cast<cuuint64_t>(a->lda)};
+  if (encode_fp8_map(&tmap_a, a->a, 2, a_dims, a_strides, static_cast<cuuint32_t>(std::min(plan.token_tile, kFp8BoxRows))) != 0) return -1;
+  const int groups = std::max(1, a->num_groups);
+  const cuuint64_t w_dims[3] = {static_cast<cuuint64_t>(a->K), static_cast<cuuint64_t>(a->N), static_cast<cuuint64_t>(groups)};
+  const cuuint64_t w_strides[2] = {static_cast<cuuint64_t>(a->ldw),
+                                   static_cast<cuuint64_t>(groups > 1 ? a->w_group_stride : a->ldw * a->N)};
+  if (encode_fp8_map(&tmap_w, a->w, 3, w_dims, w_strides, kFp8BoxRows) != 0) return -1;
+  CUDA_OK(launch_fp8_tile_gemm(tmap_a, tmap_w, p, plan.token_tile >= 128, plan.token_tile, plan.tiles, stream));
+  return 0;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+int float_size(int type) { return type == EXCHANGE_F32 ? 4 : 2; }
+
 }  // namespace
 
 extern "C" {
@@ -803,6 +913,158 @@ int b200dq_grouped_prefixes(const void* counts, int32_t counts_are_int64, int32_
   grouped_prefix_kernel<<<1, 32, 0, static_cast<cudaStream_t>(cuda_stream)>>>(
       counts, counts_are_int64, num_groups, (N + kTileRows - 1) / kTileRows, token_tile, row_prefix, tile_prefix);
   CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
+int b200dq_quant_fp8(int32_t mode, const void* x, int64_t ld_x, const void* d, int64_t ld_d, void* codes,
+                     int64_t ld_codes, float* scales, int64_t rows, int32_t cols, int32_t in_type, int32_t fp8_type,
+                     void* cuda_stream) {
+  if (mode < FP8_OF_ROWS || mode > FP8_OF_SILU_MUL_GRAD) return fail("quant_fp8: unknown mode %d", mode);
+  if (x == nullptr || codes == nullptr || scales == nullptr || (mode == FP8_OF_SILU_MUL_GRAD && d == nullptr))
+    return fail("quant_fp8: null pointer");
+  const int in_cols = mode == FP8_OF_ROWS ? 1 : 2, out_cols = mode == FP8_OF_SILU_MUL_GRAD ? 2 : 1;
+  if (rows < 0 || cols <= 0 || cols > (1 << 29)) return fail("quant_fp8: rows=%lld, cols=%d", static_cast<long long>(rows), cols);
+  if (ld_x < static_cast<int64_t>(in_cols) * cols || ld_codes < static_cast<int64_t>(out_cols) * cols ||
+      (mode == FP8_OF_SILU_MUL_GRAD && ld_d < cols))
+    return fail("quant_fp8: a row pitch is less than the row");
+  if (in_type < FP8_IN_F16 || in_type > FP8_IN_F32) return fail("quant_fp8: input must be f16, bf16 or f32");
+  if (fp8_type != FP8_E4M3 && fp8_type != FP8_E5M2) return fail("quant_fp8: result must be e4m3 or e5m2");
+  const int size = float_size(in_type);
+  if ((reinterpret_cast<uintptr_t>(x) & (size - 1)) != 0 || (reinterpret_cast<uintptr_t>(d) & (size - 1)) != 0 ||
+      (reinterpret_cast<uintptr_t>(scales) & 3) != 0)
+    return fail("quant_fp8: pointers must be aligned to their elements");
+  if (rows == 0) return 0;
+  Fp8QuantParams p;
+  memset(&p, 0, sizeof(p));
+  p.x = x; p.d = d;
+  p.codes = static_cast<uint8_t*>(codes);
+  p.scales = scales;
+  p.ld_x = ld_x; p.ld_d = ld_d; p.ld_codes = ld_codes;
+  p.rows = rows;
+  p.cols = out_cols * cols;
+  p.half = mode == FP8_OF_ROWS ? 0 : cols;
+  p.in_type = in_type; p.out_type = fp8_type;
+  p.vec = cols % (mode == FP8_OF_SILU_MUL_GRAD ? 128 : 16) == 0 && aligned16(x) && aligned16(codes) &&
+          (ld_x * size) % 16 == 0 && ld_codes % 16 == 0 &&
+          (mode != FP8_OF_SILU_MUL_GRAD || (aligned16(d) && (ld_d * size) % 16 == 0));
+  CUDA_OK(launch_fp8_quant(mode, p, static_cast<cudaStream_t>(cuda_stream)));
+  return 0;
+}
+
+int b200dq_quant_fp8_blocks(const void* x, void* codes, int64_t ld_codes, float* scales, int64_t batch, int32_t N,
+                            int32_t K, int32_t in_type, int32_t fp8_type, void* cuda_stream) {
+  if (x == nullptr || codes == nullptr || scales == nullptr) return fail("quant_fp8_blocks: null pointer");
+  if (batch <= 0 || batch > 65535 || N <= 0 || K <= 0 || (N + 127) / 128 > 65535)
+    return fail("quant_fp8_blocks: batch=%lld, N=%d, K=%d", static_cast<long long>(batch), N, K);
+  if (ld_codes < K) return fail("quant_fp8_blocks: a row pitch is less than the row");
+  if (in_type < FP8_IN_F16 || in_type > FP8_IN_F32) return fail("quant_fp8_blocks: input must be f16, bf16 or f32");
+  if (fp8_type != FP8_E4M3 && fp8_type != FP8_E5M2) return fail("quant_fp8_blocks: result must be e4m3 or e5m2");
+  if ((reinterpret_cast<uintptr_t>(x) & (float_size(in_type) - 1)) != 0 || (reinterpret_cast<uintptr_t>(scales) & 3) != 0)
+    return fail("quant_fp8_blocks: pointers must be aligned to their elements");
+  CUDA_OK(launch_fp8_quant_blocks(x, static_cast<uint8_t*>(codes), scales, batch, N, K, ld_codes, in_type, fp8_type,
+                                  static_cast<cudaStream_t>(cuda_stream)));
+  return 0;
+}
+
+int b200dq_gemm_fp8(const b200dq_fp8_gemm_args* a, void* cuda_stream) {
+  if (a == nullptr) return fail("gemm_fp8: null argument struct");
+  if (check_fp8_gemm(a) != 0) return -1;
+  DeviceState* ds = nullptr;
+  if (current_device_state(&ds) != 0) return -1;
+  return run_gemm_fp8(a, ds, static_cast<cudaStream_t>(cuda_stream));
+}
+
+size_t b200dq_exchange_scratch_bytes(int64_t tokens, int32_t top_k, int32_t num_experts) {
+  if (tokens <= 0 || top_k <= 0 || num_experts <= 0 || tokens * top_k <= kExchangeOneLaunchPairs) return 0;
+  return sizeof(int) * kExchangeMaxChunks * (static_cast<size_t>(num_experts) + 1);
+}
+
+int b200dq_exchange_dispatch(const void* experts, int32_t experts_int64, int64_t tokens, int32_t top_k,
+                             int32_t num_experts, const void* x, int64_t ld_x, int32_t width, int32_t type, void* out,
+                             int64_t ld_out, float* scales, int32_t fp8_type, int64_t* row_of, int64_t* counts,
+                             void* scratch, size_t scratch_bytes, void* cuda_stream) {
+  if (experts == nullptr || x == nullptr || out == nullptr || row_of == nullptr || counts == nullptr)
+    return fail("exchange_dispatch: null pointer");
+  if (tokens <= 0 || top_k <= 0 || width <= 0 || tokens > 0x7fffffffll / top_k)
+    return fail("exchange_dispatch: tokens=%lld, top_k=%d, width=%d (tokens * top_k must stay below 2^31)", static_cast<long long>(tokens), top_k, width);
+  if (num_experts <= 0 || num_experts > kExchangeMaxExperts) return fail("exchange_dispatch: num_experts=%d outside [1, %d]", num_experts, kExchangeMaxExperts);
+  if (type < EXCHANGE_F16 || type > EXCHANGE_F32) return fail("exchange_dispatch: rows must be f16, bf16 or f32");
+  if (scales != nullptr && fp8_type != FP8_E4M3 && fp8_type != FP8_E5M2) return fail("exchange_dispatch: result must be e4m3 or e5m2");
+  if (ld_x < width || ld_out < width) return fail("exchange_dispatch: a row pitch is less than the row");
+  if (scales == nullptr && ld_out != width) return fail("exchange_dispatch: copied rows are contiguous");
+  const int size = float_size(type);
+  if ((reinterpret_cast<uintptr_t>(x) & (size - 1)) != 0 || (scales == nullptr && (reinterpret_cast<uintptr_t>(out) & (size - 1)) != 0))
+    return fail("exchange_dispatch: pointers must be aligned to their elements");
+  if (scratch_bytes < b200dq_exchange_scratch_bytes(tokens, top_k, num_experts) ||
+      (scratch == nullptr && b200dq_exchange_scratch_bytes(tokens, top_k, num_experts) > 0))
+    return fail("exchange_dispatch: the scratch is too small");
+  ExchangeSortParams s;
+  memset(&s, 0, sizeof(s));
+  s.experts = experts;
+  s.experts_int64 = experts_int64;
+  s.tokens = tokens;
+  s.top_k = top_k; s.num_experts = num_experts;
+  s.row_of = reinterpret_cast<long long*>(row_of);
+  s.counts = reinterpret_cast<long long*>(counts);
+  s.scratch = static_cast<int*>(scratch);
+  ExchangeRowsParams r;
+  memset(&r, 0, sizeof(r));
+  r.x = x;
+  r.ld_x = ld_x;
+  r.width = width; r.type = type;
+  r.out = out;
+  r.ld_out = ld_out;
+  r.scales = scales;
+  r.fp8_type = fp8_type;
+  r.vec = aligned16(x) && aligned16(out) && (ld_x * size) % 16 == 0 &&
+          (scales != nullptr ? width % 16 == 0 && ld_out % 16 == 0 : (static_cast<long long>(width) * size) % 16 == 0);
+  CUDA_OK(launch_exchange_dispatch(s, r, static_cast<cudaStream_t>(cuda_stream)));
+  return 0;
+}
+
+int b200dq_exchange_sum(const void* y, const int64_t* row_of, const float* weights, void* out, int64_t tokens,
+                        int32_t top_k, int32_t width, int32_t type, void* cuda_stream) {
+  if (y == nullptr || row_of == nullptr || out == nullptr) return fail("exchange_sum: null pointer");
+  if (tokens < 0 || top_k <= 0 || width <= 0) return fail("exchange_sum: tokens=%lld, top_k=%d, width=%d", static_cast<long long>(tokens), top_k, width);
+  if (type < EXCHANGE_F16 || type > EXCHANGE_F32) return fail("exchange_sum: rows must be f16, bf16 or f32");
+  const int size = float_size(type);
+  if (((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out)) & (size - 1)) != 0)
+    return fail("exchange_sum: pointers must be aligned to their elements");
+  if (tokens == 0) return 0;
+  ExchangeSumParams p;
+  memset(&p, 0, sizeof(p));
+  p.y = y;
+  p.row_of = reinterpret_cast<const long long*>(row_of);
+  p.weights = weights;
+  p.out = out;
+  p.tokens = tokens;
+  p.top_k = top_k; p.width = width; p.type = type;
+  p.vec = aligned16(y) && aligned16(out) && (static_cast<long long>(width) * size) % 16 == 0;
+  CUDA_OK(launch_exchange_sum(p, static_cast<cudaStream_t>(cuda_stream)));
+  return 0;
+}
+
+int b200dq_exchange_sum_grad(const void* d_out, const void* y, const int64_t* row_of, const float* weights, void* d_y,
+                             float* d_weights, int64_t tokens, int32_t top_k, int32_t width, int32_t type,
+                             void* cuda_stream) {
+  if (d_out == nullptr || row_of == nullptr || weights == nullptr || (d_weights != nullptr && y == nullptr))
+    return fail("exchange_sum_grad: null pointer");
+  if (tokens < 0 || top_k <= 0 || width <= 0) return fail("exchange_sum_grad: tokens=%lld, top_k=%d, width=%d", static_cast<long long>(tokens), top_k, width);
+  if (type < EXCHANGE_F16 || type > EXCHANGE_F32) return fail("exchange_sum_grad: rows must be f16, bf16 or f32");
+  const int size = float_size(type);
+  if (((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(d_out) | reinterpret_cast<uintptr_t>(d_y)) & (size - 1)) != 0)
+    return fail("exchange_sum_grad: pointers must be aligned to their elements");
+  if (tokens == 0 || (d_y == nullptr && d_weights == nullptr)) return 0;
+  ExchangeSumGradParams p;
+  memset(&p, 0, sizeof(p));
+  p.d_out = d_out; p.y = y;
+  p.row_of = reinterpret_cast<const long long*>(row_of);
+  p.weights = weights;
+  p.d_y = d_y; p.d_weights = d_weights;
+  p.tokens = tokens;
+  p.top_k = top_k; p.width = width; p.type = type;
+  p.vec = aligned16(d_out) && aligned16(y) && aligned16(d_y) && (static_cast<long long>(width) * size) % 16 == 0;
+  CUDA_OK(launch_exchange_sum_grad(p, static_cast<cudaStream_t>(cuda_stream)));
   return 0;
 }
 

@@ -1,0 +1,62 @@
+// Host side of the token exchange: chunk sizes, launches.
+#include "exchange_launch.h"
+
+#include <algorithm>
+
+#include "exchange.cuh"
+
+namespace b200dq {
+
+namespace {
+
+template <typename MOVE>
+cudaError_t dispatch(const ExchangeSortParams& s, const ExchangeRowsParams& r, cudaStream_t stream) {
+  const long long pairs = s.tokens * s.top_k;
+  const int bins = s.num_experts + 1;
+  if (pairs <= kExchangeOneLaunchPairs) {
+    const int per = static_cast<int>((s.tokens + 295) / 296);              // two CTAs an SM
+    const int grid = static_cast<int>((s.tokens + per - 1) / per);
+    exchange_dispatch_small_kernel<MOVE><<<grid, 256, 2 * bins * sizeof(int), stream>>>(s, r, per);
+    return cudaGetLastError();
+  }
+  const long long per = std::max<long long>(512, (pairs + kExchangeMaxChunks - 1) / kExchangeMaxChunks);
+  const int chunks = static_cast<int>((pairs + per - 1) / per);
+  exchange_count_kernel<<<chunks, 256, bins * sizeof(int), stream>>>(s, per);
+  exchange_place_kernel<<<chunks, kPlaceWarps * 32, (kPlaceWarps + 1) * bins * sizeof(int), stream>>>(s, per);
+  const int grid = static_cast<int>(std::min<long long>(s.tokens, 148 * 32));
+  exchange_move_kernel<MOVE><<<grid, 256, 0, stream>>>(s, r);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t dispatch_quant(const ExchangeSortParams& s, const ExchangeRowsParams& r, cudaStream_t stream) {
+  return r.fp8_type == FP8_E4M3 ? dispatch<QuantMove<T, FP8_E4M3>>(s, r, stream) : dispatch<QuantMove<T, FP8_E5M2>>(s, r, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_exchange_dispatch(const ExchangeSortParams& s, const ExchangeRowsParams& r, cudaStream_t stream) {
+  if (r.scales == nullptr) return dispatch<CopyMove>(s, r, stream);
+  if (r.type == EXCHANGE_F16) return dispatch_quant<__half>(s, r, stream);
+  if (r.type == EXCHANGE_BF16) return dispatch_quant<__nv_bfloat16>(s, r, stream);
+  return dispatch_quant<float>(s, r, stream);
+}
+
+cudaError_t launch_exchange_sum(const ExchangeSumParams& p, cudaStream_t stream) {
+  const int v = p.vec ? (p.type == EXCHANGE_F32 ? 4 : 8) : 1;
+  const int grid = static_cast<int>(std::min<long long>((p.tokens * (p.width / v) + 255) / 256, 148 * 32));
+  if (p.type == EXCHANGE_F16) exchange_sum_kernel<__half><<<grid, 256, 0, stream>>>(p);
+  else if (p.type == EXCHANGE_BF16) exchange_sum_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(p);
+  else exchange_sum_kernel<float><<<grid, 256, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_exchange_sum_grad(const ExchangeSumGradParams& p, cudaStream_t stream) {
+  const int grid = static_cast<int>(std::min<long long>(p.tokens, 148 * 32));
+  if (p.type == EXCHANGE_F16) exchange_sum_grad_kernel<__half><<<grid, 256, 0, stream>>>(p);
+  else if (p.type == EXCHANGE_BF16) exchange_sum_grad_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(p);
+  else exchange_sum_grad_kernel<float><<<grid, 256, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace b200dq

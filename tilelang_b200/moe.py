@@ -9,6 +9,9 @@ weight per expert). Here the two grouped GEMMs and the activation between them a
 library's kernels; routing, the row gather and the weighted scatter-add are torch
 tensor plumbing around them.
 
+On a GPU the rows are sorted and moved by this library too (:func:`dispatch`, :func:`combine`, both
+differentiable), and :class:`Fp8ExpertMLP` runs the experts in 8-bit floating point.
+
 Expert parallelism: experts are split contiguously over the ranks, tokens start out
 partitioned by rank; one all-to-all sends every (token, expert) row to the rank that
 owns the expert, the local grouped GEMMs run, a second all-to-all returns the rows, and
@@ -17,10 +20,12 @@ GPUs, gloo in CPU tests) carries both exchanges.
 """
 from __future__ import annotations
 
-from typing import Callable, List, Optional, Sequence
+from dataclasses import dataclass
+from typing import Callable, List, Optional, Sequence, Tuple
 
 import torch
 import torch.distributed as dist
+from torch.autograd.function import once_differentiable
 
 
 def route(logits: torch.Tensor, top_k: int):
@@ -94,6 +99,174 @@ def make_gpu_expert_mlp(w1_packed, w2_packed, token_tile: Optional[int] = None) 
         return run
 
     return ExpertMLP(gemm(w1_packed), gemm(w2_packed), ops.silu_mul, ops.moe_combine)
+
+
+# ---------------------------------------------------------------------------
+# token exchange: rows sorted by expert and back, with gradients
+# ---------------------------------------------------------------------------
+
+@dataclass
+class ExchangePlan:
+    """Where every (token, slot) pair went: ``row_of`` (T, k) int64, the pair's row in expert order, or -1 - row
+    for a pair whose expert id was outside [0, E) (its row lies behind the last expert's); ``counts`` (E,)
+    int64, the rows of each expert. Both stay on the device."""
+
+    row_of: torch.Tensor
+    counts: torch.Tensor
+
+    @property
+    def tokens(self) -> int:
+        return self.row_of.shape[0]
+
+    @property
+    def top_k(self) -> int:
+        return self.row_of.shape[1]
+
+    @property
+    def num_experts(self) -> int:
+        return self.counts.numel()
+
+
+def _check_experts(x: torch.Tensor, experts: torch.Tensor, num_experts: int) -> torch.Tensor:
+    from . import ops
+    ops._check_rows("x", x)
+    if x.dtype not in ops._FLOAT_OF:
+        raise TypeError(f"x must be float16, bfloat16 or float32, got {x.dtype}")
+    if x.shape[1] == 0:
+        raise ValueError("x must have at least one column")
+    if not isinstance(experts, torch.Tensor) or experts.dtype not in (torch.int32, torch.int64):
+        raise TypeError("experts must be an int32 or int64 tensor")
+    if experts.device != x.device:
+        raise ValueError(f"experts is on {experts.device}, x on {x.device}")
+    if experts.dim() != 2 or experts.shape[0] != x.shape[0] or experts.shape[1] == 0:
+        raise ValueError(f"experts must have shape ({x.shape[0]}, top_k) with top_k at least 1, got {tuple(experts.shape)}")
+    if not 1 <= num_experts <= 1024:
+        raise ValueError(f"num_experts must lie in 1 .. 1024, got {num_experts}")
+    return experts.contiguous()
+
+
+def _exchange_out(x: torch.Tensor, experts: torch.Tensor, num_experts: int, out: torch.Tensor,
+                  scales: Optional[torch.Tensor], dtype: Optional[torch.dtype]) -> ExchangePlan:
+    """Sorts the pairs and moves the rows of ``x`` into ``out``, on the current stream."""
+    from . import _lib, ops
+    lib = _lib.load()
+    T, k = experts.shape
+    plan = ExchangePlan(torch.empty((T, k), dtype=torch.int64, device=x.device),
+                        torch.empty(num_experts, dtype=torch.int64, device=x.device))
+    if T == 0:
+        plan.counts.zero_()
+        return plan
+    ops._ensure_init(x.device)
+    need = lib.b200dq_exchange_scratch_bytes(T, k, num_experts)
+    # scratch of this call alone: calls on two streams, or in two graphs, share nothing
+    scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    with torch.cuda.device(x.device):
+        _lib.check(lib.b200dq_exchange_dispatch(
+            experts.data_ptr(), 1 if experts.dtype == torch.int64 else 0, T, k, num_experts,
+            x.data_ptr(), x.stride(0) if T > 1 else x.shape[1], x.shape[1], ops._FLOAT_OF[x.dtype], out.data_ptr(),
+            out.stride(0) if out.shape[0] > 1 else max(out.stride(0), out.shape[1]),
+            scales.data_ptr() if scales is not None else None, ops._FP8_OF[dtype] if dtype is not None else 0,
+            plan.row_of.data_ptr(), plan.counts.data_ptr(), scratch.data_ptr() if need else None, need,
+            ops._stream_ptr(x.device)), "b200dq_exchange_dispatch")
+    return plan
+
+
+class _Dispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, experts, num_experts):
+        out = torch.empty((experts.numel(), x.shape[1]), dtype=x.dtype, device=x.device)
+        plan = _exchange_out(x, experts, num_experts, out, None, None)
+        ctx.save_for_backward(plan.row_of)
+        ctx.mark_non_differentiable(plan.row_of, plan.counts)
+        ctx.set_materialize_grads(False)
+        return out, plan.row_of, plan.counts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out, _row_of, _counts):
+        if d_out is None:
+            return None, None, None
+        return _exchange_sum(d_out.contiguous(), ctx.saved_tensors[0], None), None, None
+
+
+def _exchange_sum(y: torch.Tensor, row_of: torch.Tensor, weights: Optional[torch.Tensor]) -> torch.Tensor:
+    from . import _lib, ops
+    T, k = row_of.shape
+    out = torch.empty((T, y.shape[1]), dtype=y.dtype, device=y.device)
+    if T:
+        ops._ensure_init(y.device)
+        with torch.cuda.device(y.device):
+            _lib.check(_lib.load().b200dq_exchange_sum(
+                y.data_ptr(), row_of.data_ptr(), weights.data_ptr() if weights is not None else None, out.data_ptr(),
+                T, k, y.shape[1], ops._FLOAT_OF[y.dtype], ops._stream_ptr(y.device)), "b200dq_exchange_sum")
+    return out
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, row_of, weights):
+        ctx.save_for_backward(y, row_of, weights)
+        return _exchange_sum(y, row_of, weights)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out):
+        from . import _lib, ops
+        y, row_of, weights = ctx.saved_tensors
+        T, k = row_of.shape
+        d_out = d_out.contiguous()
+        d_y = torch.empty_like(y) if ctx.needs_input_grad[0] else None
+        d_w = torch.empty_like(weights) if ctx.needs_input_grad[2] else None
+        if T:
+            with torch.cuda.device(y.device):
+                _lib.check(_lib.load().b200dq_exchange_sum_grad(
+                    d_out.data_ptr(), y.data_ptr(), row_of.data_ptr(), weights.data_ptr(),
+                    d_y.data_ptr() if d_y is not None else None, d_w.data_ptr() if d_w is not None else None,
+                    T, k, y.shape[1], ops._FLOAT_OF[y.dtype], ops._stream_ptr(y.device)), "b200dq_exchange_sum_grad")
+        return d_y, None, d_w
+
+
+def dispatch(x: torch.Tensor, experts: torch.Tensor, num_experts: int) -> Tuple[torch.Tensor, ExchangePlan]:
+    """Every token's row once for each of its experts, sorted by expert: returns ``(rows, plan)`` with rows
+    (T * k, H) in x's dtype. ``x`` (T, H) float16, bfloat16 or float32, its rows any distance apart;
+    ``experts`` (T, k) int32 or int64. Rows of one expert keep the order of their (token, slot) pairs. A pair
+    whose id lies outside [0, num_experts) -- a padded token's, say -- takes part in nothing: it gets a row of
+    zeros behind the last expert's. Differentiable in x (float32 sums over the slots, in their order)."""
+    experts = _check_experts(x, experts, num_experts)
+    rows, row_of, counts = _Dispatch.apply(x, experts, num_experts)
+    return rows, ExchangePlan(row_of, counts)
+
+
+def dispatch_fp8(x: torch.Tensor, experts: torch.Tensor, num_experts: int,
+                 dtype: torch.dtype = torch.float8_e4m3fn) -> Tuple[torch.Tensor, torch.Tensor, ExchangePlan]:
+    """:func:`dispatch` with every token quantised once on its way, as :func:`ops.quant_fp8` does it: returns
+    ``(codes (T * k, H), scales (T * k, ceil(H / 128)), plan)``. Not differentiable. A dropped pair's row has
+    zero codes."""
+    from . import ops
+    ops._check_fp8_target(dtype)
+    experts = _check_experts(x, experts, num_experts)
+    rows = experts.numel()
+    codes = ops._fp8_rows(rows, x.shape[1], dtype, x.device)
+    scales = torch.empty((rows, ops._blocks128(x.shape[1])), dtype=torch.float32, device=x.device)
+    return codes, scales, _exchange_out(x.detach(), experts, num_experts, codes, scales, dtype)
+
+
+def combine(y: torch.Tensor, plan: ExchangePlan, weights: torch.Tensor) -> torch.Tensor:
+    """Back from expert order: ``out[t] = sum_s weights[t, s] * y[plan.row_of[t, s]]``, float32 sums in slot order
+    rounded once to y's dtype; dropped pairs add nothing. ``y`` (T * k, H) contiguous float16, bfloat16 or float32,
+    ``weights`` (T, k) of any floating type. Differentiable in y and weights."""
+    from . import ops
+    ops._check_cuda_contig("y", y)
+    if y.dim() != 2 or y.dtype not in ops._FLOAT_OF:
+        raise ValueError("y must be a 2-D float16, bfloat16 or float32 tensor")
+    row_of = plan.row_of
+    if row_of.device != y.device or weights.device != y.device:
+        raise ValueError("y, the plan and the weights must be on one device")
+    if not weights.dtype.is_floating_point or weights.shape != row_of.shape:
+        raise ValueError(f"weights must be floating point of shape {tuple(row_of.shape)}, got {weights.dtype} {tuple(weights.shape)}")
+    if y.shape[0] != row_of.numel() or y.shape[1] == 0:
+        raise ValueError(f"y must have {row_of.numel()} rows of at least one column, got {tuple(y.shape)}")
+    return _Combine.apply(y, row_of, weights.float().contiguous())
 
 
 def moe_forward(x: torch.Tensor, logits: torch.Tensor, top_k: int, num_experts: int, mlp: ExpertMLP) -> torch.Tensor:

@@ -584,6 +584,282 @@ def silu_mul(h: torch.Tensor) -> torch.Tensor:
     return out
 
 
+# ---------------------------------------------------------------------------
+# 8-bit floating point with a scale for each block of 128
+# ---------------------------------------------------------------------------
+
+_FP8_OF = {torch.float8_e4m3fn: _lib.FP8_E4M3, torch.float8_e5m2: _lib.FP8_E5M2}
+_FLOAT_OF = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
+
+
+def _blocks128(n: int) -> int:
+    return (n + 127) // 128
+
+
+def _check_rows(name: str, t: torch.Tensor, device: Optional[torch.device] = None) -> int:
+    """A 2-D CUDA tensor whose rows are contiguous and do not overlap; returns their pitch in elements."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
+    if t.dim() != 2:
+        raise ValueError(f"{name} must have two dimensions, got shape {tuple(t.shape)}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} must have contiguous rows")
+    if rows > 1 and t.stride(0) < cols:
+        raise ValueError(f"{name} has rows that overlap")
+    return t.stride(0) if rows > 1 else cols
+
+
+def _fp8_rows(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """(rows, cols) codes whose row pitch is a multiple of 16 bytes, as the products read them."""
+    return torch.empty((rows, (cols + 15) // 16 * 16), dtype=dtype, device=device)[:, :cols]
+
+
+def _check_fp8_target(dtype: torch.dtype) -> None:
+    if dtype not in _FP8_OF:
+        raise TypeError(f"the codes are float8_e4m3fn or float8_e5m2, not {dtype}")
+
+
+def _quant_fp8(mode: int, what: str, x: torch.Tensor, d: Optional[torch.Tensor], dtype: torch.dtype):
+    lib = _lib.load()
+    _check_fp8_target(dtype)
+    ld_x = _check_rows("x" if mode == _lib.FP8_OF_ROWS else "h", x)
+    if x.dtype not in _FLOAT_OF:
+        raise TypeError(f"{what} takes float16, bfloat16 or float32, got {x.dtype}")
+    rows, width = x.shape
+    cols = width if mode == _lib.FP8_OF_ROWS else width // 2
+    if mode != _lib.FP8_OF_ROWS and width % 2:
+        raise ValueError("h must have an even number of columns")
+    if cols == 0:
+        raise ValueError(f"{what} needs at least one column")
+    ld_d = 0
+    if d is not None:
+        ld_d = _check_rows("d", d, x.device)
+        if d.dtype != x.dtype or tuple(d.shape) != (rows, cols):
+            raise ValueError(f"d must be {x.dtype} of shape {(rows, cols)}, got {d.dtype} {tuple(d.shape)}")
+    out_cols = 2 * cols if mode == _lib.FP8_OF_SILU_MUL_GRAD else cols
+    codes = _fp8_rows(rows, out_cols, dtype, x.device)
+    scales = torch.empty((rows, _blocks128(out_cols)), dtype=torch.float32, device=x.device)
+    if rows:
+        _ensure_init(x.device)
+        with torch.cuda.device(x.device):
+            _lib.check(lib.b200dq_quant_fp8(mode, x.data_ptr(), ld_x, d.data_ptr() if d is not None else None, ld_d,
+                                            codes.data_ptr(), codes.stride(0), scales.data_ptr(), rows, cols,
+                                            _FLOAT_OF[x.dtype], _FP8_OF[dtype], _stream_ptr(x.device)), what)
+    return codes, scales
+
+
+def quant_fp8(x: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn):
+    """(M, K) float16/bfloat16/float32 -> (codes (M, K) of ``dtype``, scales (M, ceil(K / 128)) float32):
+    one scale for each row and 128 columns, value = code * scale.
+
+    ``scale = max|x| / 448`` (57344 for e5m2), at least 2^-126; ``code = rn(x / scale)``, ties to even, with the
+    quotient taken as ``x * (1 / scale)`` in float32. A block that holds NaN or an infinity gets that as
+    its scale, so that it does not come out of a product as a finite number. Rows of ``x`` may lie any distance apart;
+    the codes' rows lie a multiple of 16 bytes apart, as :func:`gemm_fp8` reads them."""
+    return _quant_fp8(_lib.FP8_OF_ROWS, "quant_fp8", x, None, dtype)
+
+
+def silu_mul_quant_fp8(h: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn):
+    """:func:`quant_fp8` of ``silu(h[:, :F]) * h[:, F:]`` for h of shape (rows, 2F), computed in float32
+    and rounded once, to the codes."""
+    return _quant_fp8(_lib.FP8_OF_SILU_MUL, "silu_mul_quant_fp8", h, None, dtype)
+
+
+def silu_mul_backward_quant_fp8(h: torch.Tensor, d: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn):
+    """:func:`quant_fp8` of the gradient of ``silu(h[:, :F]) * h[:, F:]`` with respect to h, (rows, 2F), from
+    ``d`` (rows, F), the gradient of the product, in h's dtype."""
+    if not isinstance(d, torch.Tensor):
+        raise TypeError("d must be a torch.Tensor")
+    return _quant_fp8(_lib.FP8_OF_SILU_MUL_GRAD, "silu_mul_backward_quant_fp8", h, d, dtype)
+
+
+@dataclass
+class Fp8Weight:
+    """A weight in 8-bit floating point with one float32 scale for each block of 128 x 128: value[n, k] =
+    codes[n, k] * scales[n // 128, k // 128]. ``codes`` (N, K), or (E, N, K) for one matrix per expert;
+    ``scales`` (N blocks, K blocks) or (E, N blocks, K blocks). The kernels read it as it is."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def num_groups(self) -> int:
+        return self.codes.shape[0] if self.codes.dim() == 3 else 0
+
+    @property
+    def N(self) -> int:
+        return self.codes.shape[-2]
+
+    @property
+    def K(self) -> int:
+        return self.codes.shape[-1]
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + 4 * self.scales.numel()
+
+
+def quant_fp8_weight(w: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> Fp8Weight:
+    """(N, K) or (E, N, K) float16/bfloat16/float32 -> :class:`Fp8Weight`, by the rule of :func:`quant_fp8` over
+    blocks of 128 x 128. Offline, once per weight."""
+    lib = _lib.load()
+    _check_fp8_target(dtype)
+    _check_cuda_contig("w", w)
+    if w.dim() not in (2, 3) or w.dtype not in _FLOAT_OF:
+        raise ValueError("w must be a float16, bfloat16 or float32 tensor of two or three dimensions")
+    if w.numel() == 0:
+        raise ValueError("w must not be empty")
+    lead, (N, K) = w.shape[:-2], w.shape[-2:]
+    codes = torch.empty((*lead, N, (K + 15) // 16 * 16), dtype=dtype, device=w.device)[..., :K]
+    scales = torch.empty((*lead, _blocks128(N), _blocks128(K)), dtype=torch.float32, device=w.device)
+    _ensure_init(w.device)
+    with torch.cuda.device(w.device):
+        _lib.check(lib.b200dq_quant_fp8_blocks(w.data_ptr(), codes.data_ptr(), codes.stride(-2), scales.data_ptr(),
+                                               w.shape[0] if lead else 1, N, K, _FLOAT_OF[w.dtype], _FP8_OF[dtype],
+                                               _stream_ptr(w.device)), "b200dq_quant_fp8_blocks")
+    return Fp8Weight(codes, scales)
+
+
+def _fp8_gemm_args(what: str, a: torch.Tensor, a_scale: torch.Tensor, w: Fp8Weight, trans_w: bool, grouped: bool):
+    """Checks the operands of a product and fills the argument struct but for the output and the counts."""
+    lda = _check_rows("a", a)
+    dev = a.device
+    if a.dtype not in _FP8_OF:
+        raise TypeError(f"a must be float8_e4m3fn or float8_e5m2, got {a.dtype}")
+    codes, scales = w.codes, w.scales
+    for name, t in (("w.codes", codes), ("w.scales", scales)):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
+        if t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, a on {dev}")
+    if codes.dtype not in _FP8_OF:
+        raise TypeError(f"w.codes must be float8_e4m3fn or float8_e5m2, got {codes.dtype}")
+    if codes.dim() != (3 if grouped else 2):
+        raise ValueError(f"{what} takes w.codes of shape {'(E, N, K)' if grouped else '(N, K)'}, got {tuple(codes.shape)}")
+    N, K = codes.shape[-2:]
+    G = codes.shape[0] if grouped else 0
+    if N == 0 or K == 0 or (grouped and G == 0):
+        raise ValueError("w must not be empty")
+    inner = N if trans_w else K
+    M = a.shape[0]
+    if a.shape[1] != inner:
+        raise ValueError(f"a must have shape (M, {inner}), got {tuple(a.shape)}")
+    if K > 1 and codes.stride(-1) != 1:
+        raise ValueError("w.codes must have contiguous rows")
+    ldw = codes.stride(-2) if N > 1 else (K + 15) // 16 * 16
+    group_stride = codes.stride(0) if G > 1 else ldw * N
+    if M == 1:
+        lda = (inner + 15) // 16 * 16
+    if a.data_ptr() % 16 or lda % 16 or codes.data_ptr() % 16 or ldw % 16 or group_stride % 16:
+        raise ValueError("rows of a and w.codes must start on 16-byte boundaries (quant_fp8 and quant_fp8_weight lay them out so)")
+    if ldw < K or group_stride < ldw * N:
+        raise ValueError("w.codes has rows or matrices that overlap")
+    blocks = (_blocks128(N), _blocks128(K))
+    want = (G, *blocks) if grouped else blocks
+    if scales.dtype != torch.float32 or tuple(scales.shape) != want or not scales.is_contiguous():
+        raise ValueError(f"w.scales must be contiguous float32 of shape {want}, got {scales.dtype} {tuple(scales.shape)}")
+    ld_scale = _check_rows("a_scale", a_scale, dev)
+    if a_scale.dtype != torch.float32 or tuple(a_scale.shape) != (M, _blocks128(inner)):
+        raise ValueError(f"a_scale must be float32 of shape {(M, _blocks128(inner))}, got {a_scale.dtype} {tuple(a_scale.shape)}")
+    return _lib.Fp8GemmArgs(
+        a=a.data_ptr(), a_scale=a_scale.data_ptr(), w=codes.data_ptr(), w_scale=scales.data_ptr(),
+        lda=lda, ld_a_scale=ld_scale, ldw=ldw, w_group_stride=group_stride, M=M, N=N, K=K,
+        num_groups=G, a_type=_FP8_OF[a.dtype], w_type=_FP8_OF[codes.dtype], trans_w=1 if trans_w else 0)
+
+
+def _fp8_gemm_out(M: int, cols: int, out: Optional[torch.Tensor], out_dtype: torch.dtype, device: torch.device):
+    if out is None:
+        if out_dtype not in _FLOAT_OF:
+            raise TypeError(f"out_dtype must be float16, bfloat16 or float32, not {out_dtype}")
+        return torch.empty((M, cols), dtype=out_dtype, device=device)
+    _check_cuda_contig("out", out, device)
+    if tuple(out.shape) != (M, cols) or out.dtype not in _FLOAT_OF:
+        raise ValueError(f"out must be float16, bfloat16 or float32 of shape {(M, cols)}, got {out.dtype} {tuple(out.shape)}")
+    return out
+
+
+def _run_gemm_fp8(args, out: torch.Tensor, what: str) -> torch.Tensor:
+    if args.M == 0:
+        return out
+    lib = _lib.load()
+    args.c, args.out_type = out.data_ptr(), _OUT_OF[out.dtype]
+    _ensure_init(out.device)
+    with torch.cuda.device(out.device):
+        _lib.check(lib.b200dq_gemm_fp8(ctypes.byref(args), _stream_ptr(out.device)), what)
+    return out
+
+
+def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: Fp8Weight, trans_w: bool = False,
+             out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16, token_tile: int = 0,
+             split: int = 0) -> torch.Tensor:
+    """``C = A @ W^T`` with ``a`` (M, K) codes and ``a_scale`` (M, ceil(K / 128)) from :func:`quant_fp8`, ``w`` an
+    (N, K) :class:`Fp8Weight`; C is (M, N) in float16, bfloat16 or float32. With ``trans_w`` it is
+    ``C = A @ W`` with ``a`` (M, N): the gradient of the input, (M, K), from the same weight.
+    The two operands may be of different 8-bit types. Sums are float32 throughout, the result is rounded once.
+    ``token_tile`` (16, 32, 64 or 128) and ``split`` (1 to 8) override the kernel's tile and the CTAs that
+    share its contraction; 0 leaves them to the library."""
+    args = _fp8_gemm_args("gemm_fp8", a, a_scale, w, trans_w, grouped=False)
+    out = _fp8_gemm_out(a.shape[0], w.K if trans_w else w.N, out, out_dtype, a.device)
+    args.token_tile, args.split = token_tile, split
+    return _run_gemm_fp8(args, out, "b200dq_gemm_fp8")
+
+
+def _device_counts(counts, groups: int, rows: int, device: torch.device) -> torch.Tensor:
+    if isinstance(counts, torch.Tensor):
+        if counts.device != device or counts.dtype not in (torch.int32, torch.int64) or not counts.is_contiguous():
+            raise ValueError("counts must be a host sequence or a contiguous int32/int64 tensor on a's device")
+        if counts.dim() != 1 or counts.numel() != groups:
+            raise ValueError(f"counts must have one entry per expert ({groups})")
+        return counts
+    counts = [int(c) for c in counts]
+    if len(counts) != groups:
+        raise ValueError(f"counts must have one entry per expert ({groups})")
+    if min(counts) < 0 or sum(counts) > rows:
+        raise ValueError(f"counts must be non-negative and sum to at most a's {rows} rows")
+    return torch.tensor(counts, dtype=torch.int64).to(device, non_blocking=True)
+
+
+def gemm_fp8_grouped(a: torch.Tensor, a_scale: torch.Tensor, w: Fp8Weight, counts, trans_w: bool = False,
+                     out: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16,
+                     token_tile: int = 0, split: int = 0) -> torch.Tensor:
+    """:func:`gemm_fp8` for rows sorted by expert: expert e has ``counts[e]`` rows and multiplies its own matrix
+    of ``w`` (codes (E, N, K)). ``counts``: a host sequence, or an int32/int64 tensor on the device, which the
+    kernel reads there. Rows behind the last expert's are left as they are in ``out`` (undefined where it is
+    allocated here); device counts that ask for more rows than ``a`` has are cut off."""
+    args = _fp8_gemm_args("gemm_fp8_grouped", a, a_scale, w, trans_w, grouped=True)
+    counts = _device_counts(counts, w.num_groups, a.shape[0], a.device)
+    out = _fp8_gemm_out(a.shape[0], w.K if trans_w else w.N, out, out_dtype, a.device)
+    args.counts, args.counts_int64 = counts.data_ptr(), 1 if counts.dtype == torch.int64 else 0
+    args.token_tile, args.split = token_tile, split
+    return _run_gemm_fp8(args, out, "b200dq_gemm_fp8 (grouped)")
+
+
+def gemm_fp8_gated(a: torch.Tensor, a_scale: torch.Tensor, w: Fp8Weight, counts=None,
+                   dtype: torch.dtype = torch.float8_e4m3fn, keep_h: bool = False):
+    """The first product of a gated MLP with its activation, quantised for the second one: with
+    ``h = A @ W^T`` (``w`` of 2F rows, or (E, 2F, K) with ``counts``), returns the codes and scales of
+    ``silu(h[:, :F]) * h[:, F:]`` as :func:`silu_mul_quant_fp8` gives them for h in float32. With ``keep_h`` it returns
+    ``(codes, scales, h)``, h rounded to bfloat16, for the backward pass. Rows behind the last expert's
+    are undefined."""
+    _check_fp8_target(dtype)
+    if w.N % 2:
+        raise ValueError("w must have an even number of rows: gate above up")
+    if counts is None:
+        h = gemm_fp8(a, a_scale, w, out_dtype=torch.float32)
+    else:
+        h = gemm_fp8_grouped(a, a_scale, w, counts, out_dtype=torch.float32)
+    codes, scales = silu_mul_quant_fp8(h, dtype)
+    return (codes, scales, h.to(torch.bfloat16)) if keep_h else (codes, scales)
+
+
 def check_status(device: Optional[torch.device] = None) -> None:
     """Raise if a kernel recorded a device-side error (a bounded wait that gave up)."""
     dev = device or torch.device("cuda", torch.cuda.current_device())
