@@ -185,7 +185,20 @@ def test_every_tile_and_split(token_tile, split, trans):
     check_product(c, a, a_scale, w.codes, w.scales, trans)
 
 
-@pytest.mark.parametrize("token_tile", [16, 32, 64, 128])
+@pytest.mark.parametrize("M,N,K", [(1, 100, 64), (128, 256, 128), (129, 300, 400), (700, 656, 1100), (2500, 1600, 160)])
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_tiles_of_cta_pairs(M, N, K, trans, out_dtype):
+    """Pairs with one row, an empty half, several tiles to a pair, more blocks than stages."""
+    M, N, K = (M, K, N) if trans and K % 16 == 0 else (M, N, K)
+    a, a_scale, w = operands(M, N, K, 13, trans=trans)
+    c = ops.gemm_fp8(a, a_scale, w, trans_w=trans, out_dtype=out_dtype, token_tile=256)
+    tb.check_status()
+    check_product(c, a, a_scale, w.codes, w.scales, trans)
+    assert torch.equal(c, ops.gemm_fp8(a, a_scale, w, trans_w=trans, out_dtype=out_dtype, token_tile=256))
+
+
+@pytest.mark.parametrize("token_tile", [16, 32, 64, 128, 256])
 @pytest.mark.parametrize("trans", [False, True])
 def test_one_hot_rows_read_the_weight_back(token_tile, trans):
     """A row of one 1 and scales that are powers of two give the weight's values, bit for bit."""
@@ -227,7 +240,7 @@ def test_infinities_stay_in_their_rows():
     x[3, 5], x[7, 300] = float("inf"), float("nan")
     a, a_scale = ops.quant_fp8(x)
     w = ops.quant_fp8_weight(randn(256, 512, seed=4))
-    for tile in (16, 32, 64, 128):
+    for tile in (16, 32, 64, 128, 256):
         c = ops.gemm_fp8(a, a_scale, w, token_tile=tile)
         bad = torch.zeros(40, dtype=torch.bool, device=DEV)
         bad[[3, 7]] = True
@@ -253,7 +266,7 @@ COUNTS = [[1], [0, 3, 0], [300, 0, 17, 256, 1], [40, 90, 33], [1] * 40, [0] * 35
 
 @pytest.mark.parametrize("counts", COUNTS)
 @pytest.mark.parametrize("trans", [False, True])
-@pytest.mark.parametrize("token_tile", [0, 16, 64, 128])
+@pytest.mark.parametrize("token_tile", [0, 16, 64, 128, 256])
 def test_grouped_product(counts, trans, token_tile):
     """Empty experts, single rows, exact tiles; rows behind the last expert stay as they were."""
     N, K = 144, 272
@@ -270,7 +283,7 @@ def test_grouped_product(counts, trans, token_tile):
         assert (out[at:] == 7.0).all()
 
 
-@pytest.mark.parametrize("token_tile", [0, 16, 128])
+@pytest.mark.parametrize("token_tile", [0, 16, 128, 256])
 def test_device_counts_that_ask_for_more_rows_than_there_are(token_tile):
     a, a_scale, w = grouped_operands([100, 60], 256, 256, 3)
     want = ops.gemm_fp8_grouped(a, a_scale, w, [100, 60], token_tile=token_tile)

@@ -492,7 +492,7 @@ int run_gemm(const char* who, const b200dq_gemm_args* a, void* scratch, size_t s
 // ---- block-scaled fp8 products ---------------------------------------------------------------
 
 struct Fp8Plan {
-  int token_tile;        // 16, 32, 64: tokens in columns; 128: tokens on lanes
+  int token_tile;        // 16, 32, 64: tokens in columns; 128: tokens on lanes; 256: CTA pairs
   int split;
   long long tiles;       // clusters to launch (an upper bound when the counts are on the device)
 };
@@ -508,6 +508,10 @@ Fp8Plan plan_fp8(int rows, int groups, int p_tiles, int q_blocks, int sms, int t
   Fp8Plan plan;
   const long long share = groups > 0 ? (rows + groups - 1) / groups : rows;
   plan.token_tile = token_tile > 0 ? token_tile : share <= 16 ? 16 : share <= 32 ? 32 : share <= 64 ? 64 : 128;
+  if (token_tile == 0 && share > 128 && groups <= kFp8PairMaxGroups &&
+      static_cast<long long>((rows + 255) / 256) * ((p_tiles + 1) / 2) * 2 >= sms / 2)
+    plan.token_tile = 256;
+  if (plan.token_tile == 256) p_tiles = (p_tiles + 1) / 2;
   long long token_tiles = (rows + plan.token_tile - 1) / plan.token_tile;
   if (groups > 0) token_tiles = rows / plan.token_tile + std::min<long long>(groups, rows);
   plan.tiles = token_tiles * p_tiles;
@@ -548,8 +552,12 @@ int check_fp8_gemm(const b200dq_fp8_gemm_args* a) {
   if ((reinterpret_cast<uintptr_t>(a->a_scale) & 3) != 0 || (reinterpret_cast<uintptr_t>(a->w_scale) & 3) != 0 ||
       (reinterpret_cast<uintptr_t>(a->c) & (out_elem_size(a->out_type) - 1)) != 0)
     return fail("gemm_fp8: scales and output must be aligned to their elements");
-  if (a->token_tile != 0 && a->token_tile != 16 && a->token_tile != 32 && a->token_tile != 64 && a->token_tile != 128)
-    return fail("gemm_fp8: token_tile must be 0, 16, 32, 64 or 128 (got %d)", a->token_tile);
+  if (a->token_tile != 0 && a->token_tile != 16 && a->token_tile != 32 && a->token_tile != 64 && a->token_tile != 128 &&
+      a->token_tile != 256)
+    return fail("gemm_fp8: token_tile must be 0, 16, 32, 64, 128 or 256 (got %d)", a->token_tile);
+  if (a->token_tile == 256 && a->num_groups > kFp8PairMaxGroups)
+    return fail("gemm_fp8: the 256-token tile takes at most %d groups", kFp8PairMaxGroups);
+  if (a->token_tile == 256 && a->split > 1) return fail("gemm_fp8: the 256-token tile does not split the contraction");
   if (a->split < 0 || a->split > 8) return fail("gemm_fp8: split must be 0 to 8 (got %d)", a->split);
   return 0;
 }
@@ -574,6 +582,7 @@ int run_gemm_fp8(const b200dq_fp8_gemm_args* a, const DeviceState* ds, cudaStrea
   p.a_fmt = a->a_type; p.w_fmt = a->w_type;
   p.trans_w = a->trans_w ? 1 : 0;
   p.c_vec = outer % 4 == 0 && (reinterpret_cast<uintptr_t>(a->c) & (4 * out_elem_size(a->out_type) - 1)) == 0;
+  p.c_vec16 = (outer * out_elem_size(a->out_type)) % 16 == 0 && (reinterpret_cast<uintptr_t>(a->c) & 15) == 0;
   p.counts = a->num_groups > 0 ? a->counts : nullptr;
   p.counts_int64 = a->counts_int64;
   p.num_groups = a->num_groups;
@@ -589,6 +598,11 @@ int run_gemm_fp8(const b200dq_fp8_gemm_args* a, const DeviceState* ds, cudaStrea
   const cuuint64_t w_strides[2] = {static_cast<cuuint64_t>(a->ldw),
                                    static_cast<cuuint64_t>(groups > 1 ? a->w_group_stride : a->ldw * a->N)};
   if (encode_fp8_map(&tmap_w, a->w, 3, w_dims, w_strides, kFp8BoxRows) != 0) return -1;
+  if (plan.token_tile == 256) {
+    p.p_tiles = (p.p_tiles + 1) / 2;
+    CUDA_OK(launch_fp8_pair_gemm(tmap_a, tmap_w, p, static_cast<int>(std::min<long long>(plan.tiles, ds->sm_count / 2)), stream));
+    return 0;
+  }
   CUDA_OK(launch_fp8_tile_gemm(tmap_a, tmap_w, p, plan.token_tile >= 128, plan.token_tile, plan.tiles, stream));
   return 0;
 }

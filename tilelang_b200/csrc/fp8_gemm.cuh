@@ -271,7 +271,7 @@ fp8_tile_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
             sc[2 * j + 1] = fmul2(pack2f(q.z, q.w), ls);
           }
         }
-        tc_wait_ld();
+        tc_wait_ld(v);
         if (c + kChunk == C::kCols) {
           // the accumulator (and the scales) go back before the last additions
           tc_fence_before_sync();

@@ -2,6 +2,7 @@
 #include "fp8_launch.h"
 
 #include "fp8_gemm.cuh"
+#include "fp8_pair_gemm.cuh"
 
 namespace b200dq {
 
@@ -51,6 +52,23 @@ cudaError_t launch_fp8_tile_gemm(const CUtensorMap& tmap_a, const CUtensorMap& t
     case 64: return launch_tile<false, 64>(tmap_a, tmap_w, p, tiles, stream);
     default: return cudaErrorInvalidValue;
   }
+}
+
+cudaError_t launch_fp8_pair_gemm(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const Fp8GemmParams& p, int pairs,
+                                 cudaStream_t stream) {
+  static_assert(kFp8PairMaxGroups == kPairMaxGroups, "tile table");
+  static bool attr_set[kMaxDevices] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  if (!attr_set[dev]) {
+    e = cudaFuncSetAttribute(fp8_pair_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes);
+    if (e != cudaSuccess) return e;
+    attr_set[dev] = true;
+  }
+  fp8_pair_gemm_kernel<<<2 * pairs, kPairThreads, kPairSmemBytes, stream>>>(tmap_a, tmap_w, p);
+  return cudaGetLastError();
 }
 
 }  // namespace b200dq

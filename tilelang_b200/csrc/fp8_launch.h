@@ -23,6 +23,7 @@ struct Fp8GemmParams {
   int a_fmt, w_fmt;          // FP8_E4M3 / FP8_E5M2
   int trans_w;
   int c_vec;                 // four columns may be stored at once
+  int c_vec16;               // 16 bytes may be stored at once
   const void* counts;        // grouped: rows of each group, on the device; null: one group of M rows
   int counts_int64, num_groups;
   int split;                 // CTAs of a cluster that share a tile's contraction
@@ -35,5 +36,10 @@ constexpr int kFp8BoxRows = 128;    // rows of a weight box, and of a token box 
 // Tokens own the accumulator's 128 lanes (tokens_on_lanes) or its columns, `tile_tokens` (16, 32, 64, 128) of them.
 cudaError_t launch_fp8_tile_gemm(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const Fp8GemmParams& p,
                                  bool tokens_on_lanes, int tile_tokens, long long tiles, cudaStream_t stream);
+
+// CTA pairs, 256 tokens x 256 columns (p.p_tiles counts tiles of 256); `pairs` clusters of two.
+cudaError_t launch_fp8_pair_gemm(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const Fp8GemmParams& p, int pairs,
+                                 cudaStream_t stream);
+constexpr int kFp8PairMaxGroups = 256;
 
 }  // namespace b200dq

@@ -1,0 +1,295 @@
+// The product of fp8_gemm.cuh for many tokens: CTA pairs, tiles of 256 tokens x 256 weight rows.
+//
+// A pair of CTAs on two SMs works on one tile with tcgen05.mma.cta_group::2 (M = N = 256): each CTA
+// loads 128 tokens and 128 weight rows per block of 128, 32 KB for 8.4 million multiply-adds, half of
+// what a CTA on its own would pull through L2 for the same work (at 128 x 256 the crossbar would
+// carry 14 TB/s at the tensor cores' rate). Its 128 x 256 sums per block go to one of two accumulators that
+// fill tensor memory, and eight warps move them, scaled, to fp32 registers: thread = one token, 128
+// columns, one scale per block. 64 packed fmas a thread and block are 256 cycles of the fp32 pipe,
+// and reading tensor memory about as many, under 512 cycles of multiplication.
+//
+// Persistent: one pair per two SMs, tiles in strips of eight token tiles so that the tiles in flight
+// share their operands in L2. warp 0: TMA producer (both CTAs); warp 1: MMA issuer (first CTA);
+// warps 2, 3: tensor memory, tile table; warps 4-11: sums and output. Finished rows go through 4 KB of
+// shared memory per warp, so that a store instruction writes whole 128-byte pieces.
+#pragma once
+#include "fp8_gemm.cuh"
+
+namespace b200dq {
+
+constexpr int kPairThreads = 384;
+constexpr int kPairStages = 6;
+constexpr int kPairHalf = 128 * 128;                          // one operand's half tile: 128 rows x 128 bytes
+constexpr int kPairStageBytes = 2 * kPairHalf;
+constexpr int kPairStageOut = 32 * 128;                       // a warp's output rows, 128 bytes each
+constexpr int kPairStrip = 8;
+constexpr int kPairMaxGroups = 256;                           // groups whose tile table fits the control block
+// setmaxnreg moves registers from warps 0-3 to the eight summing warps: 128 * 40 + 256 * 232 = 384 * 168
+constexpr int kPairOtherRegs = 40, kPairSumRegs = 232;
+
+struct Fp8PairCtl {
+  uint64_t full[kPairStages], empty[kPairStages];
+  uint64_t acc_full[2], acc_empty[2];
+  uint32_t tmem_base;
+  int abort_flag;
+  int row_prefix[kPairMaxGroups + 1];
+  int tile_prefix[kPairMaxGroups + 1];                        // token tiles before each group
+};
+constexpr int kPairSmemBytes = kPairStages * kPairStageBytes + 8 * kPairStageOut +
+                               static_cast<int>((sizeof(Fp8PairCtl) + 15) / 16 * 16);
+static_assert(kPairSmemBytes <= 232448, "shared memory of a CTA");
+
+// Row and token-tile prefixes of the groups, by one warp. Counts are cut off at M rows in all.
+__device__ __forceinline__ void fp8_pair_prefixes(const Fp8GemmParams& p, Fp8PairCtl* ctl, int lane) {
+  long long rows = 0;
+  int tiles = 0;
+  for (int base = 0; base < p.num_groups; base += 32) {
+    const int g = base + lane;
+    long long c = 0;
+    if (g < p.num_groups)
+      c = p.counts_int64 ? static_cast<const long long*>(p.counts)[g] : static_cast<const int*>(p.counts)[g];
+    long long r = min(max(c, 0ll), static_cast<long long>(p.M));
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, r, d);
+      if (lane >= d) r += u;
+    }
+    const long long end = min(rows + r, static_cast<long long>(p.M));
+    long long begin = __shfl_up_sync(0xffffffffu, end, 1);
+    if (lane == 0) begin = min(rows, static_cast<long long>(p.M));
+    int n = static_cast<int>((end - begin + 255) / 256);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, n, d);
+      if (lane >= d) n += u;
+    }
+    if (g < p.num_groups) {
+      ctl->row_prefix[g + 1] = static_cast<int>(end);
+      ctl->tile_prefix[g + 1] = tiles + n;
+    }
+    rows += __shfl_sync(0xffffffffu, r, 31);
+    tiles += __shfl_sync(0xffffffffu, n, 31);
+  }
+  if (lane == 0) ctl->row_prefix[0] = ctl->tile_prefix[0] = 0;
+}
+
+// Where tile t lies: strips of kPairStrip token tiles, within a strip token tiles fastest.
+__device__ __forceinline__ Fp8Tile fp8_pair_tile(const Fp8GemmParams& p, const Fp8PairCtl* ctl, int token_tiles, long long t) {
+  const long long strip_tiles = static_cast<long long>(kPairStrip) * p.p_tiles;
+  const int strip = static_cast<int>(t / strip_tiles);
+  const int in_strip = static_cast<int>(t - strip * strip_tiles);
+  const int high = min(kPairStrip, token_tiles - strip * kPairStrip);
+  const int tt = strip * kPairStrip + in_strip % high;
+  const int p0 = in_strip / high * 256;
+  if (p.counts == nullptr) return Fp8Tile{0, tt * 256, p.M, p0};
+  int lo = 0, hi = p.num_groups;                              // tile_prefix[lo] <= tt < tile_prefix[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (ctl->tile_prefix[mid] <= tt) lo = mid; else hi = mid;
+  }
+  return Fp8Tile{lo, ctl->row_prefix[lo] + (tt - ctl->tile_prefix[lo]) * 256, ctl->row_prefix[lo + 1], p0};
+}
+
+// 32 rows x 128 columns of fp32 sums (thread = row) to C, 128 bytes of each row at a time through the
+// warp's 4 KB of shared memory (16-byte chunks rotated by the row: no bank conflicts either way).
+template <int OUT_TYPE>
+__device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, uint8_t* stage, const uint64_t (&acc)[64],
+                                               long long m_first, int rows, int col0, int lane) {
+  constexpr int kSize = OUT_TYPE == OUT_F32 ? 4 : 2;
+  constexpr int kCols = 128 / kSize;                          // columns of a pass
+#pragma unroll
+  for (int pass = 0; pass < 128 / kCols; ++pass) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {                             // 16-byte chunks of this thread's row
+      uint4 v;
+      if (OUT_TYPE == OUT_F32) {
+        const float2 a = unpack2(acc[pass * 16 + 2 * j]), b = unpack2(acc[pass * 16 + 2 * j + 1]);
+        v = make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+      } else {
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = unpack2(acc[pass * 32 + 4 * j + i]);
+          h[i] = OUT_TYPE == OUT_BF16 ? bf162_as_u32(__floats2bfloat162_rn(f.x, f.y)) : h2_as_u32(__floats2half2_rn(f.x, f.y));
+        }
+        v = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+      *reinterpret_cast<uint4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = v;
+    }
+    __syncwarp();
+    const int chunk = lane & 7;
+    const int col = col0 + pass * kCols + chunk * (16 / kSize);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = i * 4 + (lane >> 3);
+      const uint4 v = *reinterpret_cast<const uint4*>(stage + row * 128 + ((chunk ^ (row & 7)) << 4));
+      if (row < rows && col < p.P) {
+        uint8_t* dst = static_cast<uint8_t*>(p.c) + (static_cast<size_t>(m_first + row) * p.ldc + col) * kSize;
+        if (p.c_vec16) {
+          *reinterpret_cast<uint4*>(dst) = v;
+        } else {
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 16 / kSize; ++e) {
+            if (col + e >= p.P) break;
+            if (kSize == 4) reinterpret_cast<uint32_t*>(dst)[e] = w[e];
+            else reinterpret_cast<uint16_t*>(dst)[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+          }
+        }
+      }
+    }
+    __syncwarp();
+  }
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
+                     const Fp8GemmParams p) {
+  extern __shared__ __align__(1024) uint8_t fp8_pair_smem[];     // swizzle atoms start on 1 KiB boundaries
+  uint8_t* smem = fp8_pair_smem;
+  uint8_t* stage_out = smem + kPairStages * kPairStageBytes;
+  auto* ctl = reinterpret_cast<Fp8PairCtl*>(stage_out + 8 * kPairStageOut);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = &ctl->abort_flag;
+  DeviceStatus* st = p.status;
+  const int rank = static_cast<int>(cluster_rank());
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kPairStages; ++i) { mbar_init(&ctl->full[i], 1); mbar_init(&ctl->empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&ctl->acc_full[i], 1); mbar_init(&ctl->acc_empty[i], 16); }
+    ctl->abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmap_a);
+    tma_prefetch_desc(&tmap_w);
+  }
+  if (warp == 3 && p.counts != nullptr) fp8_pair_prefixes(p, ctl, lane);
+  if (warp == 2) {
+    tmem_alloc_pair(&ctl->tmem_base, 512);
+    tmem_relinquish_pair();
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  cluster_sync_all();                                         // the peer's barriers exist
+  tc_fence_after_sync();
+  const uint32_t tmem_base = ctl->tmem_base;
+  const int token_tiles = p.counts != nullptr ? ctl->tile_prefix[p.num_groups] : (p.M + 255) / 256;
+  const long long tiles = static_cast<long long>(token_tiles) * p.p_tiles;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairOtherRegs));
+    if (warp == 0 && lane == 0) {
+      // ---------------- producer: this CTA's halves, completing on the first CTA's barriers ----------------
+      uint32_t s = 0, phase = 0;
+      bool ok = true;
+      for (long long t = pair; ok && t < tiles; t += pairs) {
+        const Fp8Tile tile = fp8_pair_tile(p, ctl, token_tiles, t);
+        const int m0 = tile.m0 + rank * 128, p0 = tile.p0 + rank * 128;
+        for (int kb = 0; kb < p.q_blocks; ++kb) {
+          ok = mbar_wait_cluster(&ctl->empty[s], phase ^ 1u, abort_flag, st, 11);
+          if (!ok) break;
+          uint8_t* stage = smem + s * kPairStageBytes;
+          const uint32_t bar = cluster_map(smem_u32(&ctl->full[s]), 0);
+          if (rank == 0) mbar_arrive_expect_tx(&ctl->full[s], 2 * kPairStageBytes);
+          tma_load_2d_pair(stage, &tmap_a, kb * 128, m0, bar);
+          if (p.trans_w) tma_load_3d_pair(stage + kPairHalf, &tmap_w, p0, kb * 128, tile.group, bar);
+          else tma_load_3d_pair(stage + kPairHalf, &tmap_w, kb * 128, p0, tile.group, bar);
+          if (++s == kPairStages) { s = 0; phase ^= 1u; }
+        }
+      }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+      // ---------------- MMA issuer for both CTAs ----------------
+      const uint32_t idesc = make_idesc_f8(p.a_fmt, p.w_fmt, 0, p.trans_w, 256, 256);
+      const uint64_t w_step = p.trans_w ? 32 * 128 / 16 : 2;
+      uint32_t s = 0, phase = 0, i = 0;
+      bool ok = true;
+      for (long long t = pair; t < tiles; t += pairs) {
+        for (int kb = 0; kb < p.q_blocks; ++kb, ++i) {
+          const uint32_t buf = i & 1u;
+          ok = ok && mbar_wait_cluster(&ctl->acc_empty[buf], ((i >> 1) & 1u) ^ 1u, abort_flag, st, 12);
+          ok = ok && mbar_wait_cluster(&ctl->full[s], phase, abort_flag, st, 13);
+          tc_fence_after_sync();
+          if (ok) {
+            const uint32_t stage = smem_u32(smem + s * kPairStageBytes);
+            const uint64_t a_desc = make_smem_desc_sw128(stage), w_desc = make_smem_desc_sw128(stage + kPairHalf);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              umma_pair_ss_f8(tmem_base + buf * 256, a_desc + 2 * j, w_desc + j * w_step, idesc, j != 0);
+          }
+          tc_commit_pair(&ctl->empty[s]);
+          tc_commit_pair(&ctl->acc_full[buf]);
+          if (++s == kPairStages) { s = 0; phase ^= 1u; }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairSumRegs));
+    // ---------------- sums: thread = one token of this CTA, 128 of the tile's columns ----------------
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    uint8_t* stage = stage_out + (warp - 4) * kPairStageOut;
+    uint32_t empty_bar[2];
+    for (int b = 0; b < 2; ++b) empty_bar[b] = cluster_map(smem_u32(&ctl->acc_empty[b]), 0);
+    uint32_t i = 0;
+    bool ok = true;
+    for (long long t = pair; t < tiles; t += pairs) {
+      const Fp8Tile tile = fp8_pair_tile(p, ctl, token_tiles, t);
+      const int m_first = tile.m0 + rank * 128 + quarter * 32;
+      const int p_block = min(tile.p0 / 128 + half, (p.P - 1) / 128);       // a tile may end before its second half
+      const float* as = p.a_scale + static_cast<long long>(min(m_first + lane, p.M - 1)) * p.ld_a_scale;
+      const float* ws = p.w_scale + tile.group * p.ws_group + p_block * p.ws_p;
+      uint64_t acc[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) acc[j] = 0;
+      // the scales two blocks ahead: their latency is longer than a block's multiplication
+      float s0 = as[0] * ws[0], s1 = p.q_blocks > 1 ? as[1] * ws[p.ws_q] : 0.f;
+      for (int kb = 0; kb < p.q_blocks; ++kb, ++i) {
+        const uint32_t buf = i & 1u;
+        float a2 = 0.f, w2 = 0.f;
+        if (kb + 2 < p.q_blocks) { a2 = as[kb + 2]; w2 = ws[(kb + 2) * p.ws_q]; }
+        const uint64_t scale = pack2f(s0, s0);
+        ok &= mbar_wait_warp(&ctl->acc_full[buf], (i >> 1) & 1u, abort_flag, st, 14, lane);
+        tc_fence_after_sync();
+        const uint32_t addr = tmem_base + lane_addr + buf * 256 + half * 128;
+        uint32_t v[2][32];
+        tmem_ld_32x32b_x32(addr, v[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tc_wait_ld(v[c & 1]);
+          if (c < 3) tmem_ld_32x32b_x32(addr + (c + 1) * 32, v[(c + 1) & 1]);
+          if (c == 3) {
+            // the accumulator goes back before the last additions
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(empty_bar[buf]);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            acc[c * 16 + j] = ffma2(pack2(v[c & 1][2 * j], v[c & 1][2 * j + 1]), scale, acc[c * 16 + j]);
+        }
+        s0 = s1;
+        s1 = a2 * w2;
+      }
+      if (ok) {
+        const int rows = min(32, tile.m_end - m_first);
+        const int col0 = tile.p0 + half * 128;
+        if (p.out_type == OUT_BF16) fp8_pair_store<OUT_BF16>(p, stage, acc, m_first, rows, col0, lane);
+        else if (p.out_type == OUT_F16) fp8_pair_store<OUT_F16>(p, stage, acc, m_first, rows, col0, lane);
+        else fp8_pair_store<OUT_F32>(p, stage, acc, m_first, rows, col0, lane);
+      }
+    }
+  }
+
+  if (*abort_flag) {
+    // copies in flight land before the shared memory goes away
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  cluster_sync_all();                                         // neither CTA leaves while the other may use its memory
+  tc_fence_after_sync();
+  if (warp == 2) tmem_dealloc_pair(tmem_base, 512);
+}
+
+}  // namespace b200dq
