@@ -293,6 +293,13 @@ typedef struct b200dq_fp8_gemm_args {
   int32_t trans_w;
   int32_t token_tile;       /* 0: chosen; 16, 32, 64: tokens are the tile's columns, 128: its lanes, 256: a CTA pair's */
   int32_t split;            /* 0: chosen; else CTAs (1 to 8) that share a tile's contraction  */
+  /* Gated (NULL for none): N = 2F rows of W, gate above up, F a multiple of 128. Instead of h = A * W^T
+   * the codes and scales of silu(h[:, :F]) * h[:, F:] are written, from the fp32 sums; c may be NULL,
+   * or takes h in bf16. */
+  void* gate_codes;         /* (M, F), rows of ld_gate bytes                                   */
+  float* gate_scales;       /* (M, F / 128), contiguous                                        */
+  int64_t ld_gate;
+  int32_t gate_type;        /* enum b200dq_fp8_type                                            */
 } b200dq_fp8_gemm_args;
 
 /* Sums are fp32: exact products added on the tensor cores within a block of 128, blocks scaled and
@@ -300,6 +307,11 @@ typedef struct b200dq_fp8_gemm_args {
  * 16 bytes (c: of its element size). Deterministic; no scratch. Grouped: counts that do not sum to M
  * are clamped to the rows that exist, and rows of C behind the last group are not written. */
 int b200dq_gemm_fp8(const b200dq_fp8_gemm_args* args, void* cuda_stream);
+
+/* 1 if a gated product of these sizes is best fused (the library would take the 256-token tile for
+ * it), 0 if its rows are so few, or its halves so ragged, that the product in fp32 and
+ * b200dq_quant_fp8 are the way. */
+int b200dq_fp8_gated_fuses(int32_t M, int32_t N, int32_t K, int32_t num_groups);
 
 /* ---- token exchange of a mixture-of-experts layer ---------------------------------------
  * experts (tokens, top_k), int32 or int64: row_of[t, s] = rows of smaller experts + earlier pairs (in

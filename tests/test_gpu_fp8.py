@@ -297,12 +297,12 @@ def test_device_counts_that_ask_for_more_rows_than_there_are(token_tile):
 
 
 @pytest.mark.parametrize("F", [128, 200, 384])
-@pytest.mark.parametrize("counts", [None, [30, 0, 45, 1], [300, 140, 0, 77]])
+@pytest.mark.parametrize("counts", [None, [30, 0, 45, 1], [300, 140, 0, 77], [4000, 0, 1, 3900], 7000])
 @pytest.mark.parametrize("dtype", [E4M3, E5M2])
 def test_gated_product(F, counts, dtype):
     """The codes stand for the exact activation to half a step and what the product's own bound moves it by."""
     K = 400
-    rows = 70 if counts is None else sum(counts)
+    counts, rows = (None, counts) if isinstance(counts, int) else (counts, 70 if counts is None else sum(counts))
     a, a_scale = ops.quant_fp8(randn(rows, K, seed=F))
     x = randn(*(() if counts is None else (len(counts),)), 2 * F, K, seed=F + 1, scale=0.05)
     w = ops.quant_fp8_weight(x)

@@ -46,6 +46,7 @@ EXPORTED_SYMBOLS = (
     "b200dq_quant_fp8",
     "b200dq_quant_fp8_blocks",
     "b200dq_gemm_fp8",
+    "b200dq_fp8_gated_fuses",
     "b200dq_exchange_scratch_bytes",
     "b200dq_exchange_dispatch",
     "b200dq_exchange_sum",
@@ -116,6 +117,10 @@ class Fp8GemmArgs(ctypes.Structure):
         ("trans_w", ctypes.c_int32),
         ("token_tile", ctypes.c_int32),
         ("split", ctypes.c_int32),
+        ("gate_codes", ctypes.c_void_p),
+        ("gate_scales", ctypes.c_void_p),
+        ("ld_gate", ctypes.c_int64),
+        ("gate_type", ctypes.c_int32),
     ]
 
 
@@ -172,6 +177,8 @@ def _declare(lib):
     lib.b200dq_quant_fp8_blocks.argtypes = [vp, vp, i64, vp, i64, i32, i32, i32, i32, vp]
     lib.b200dq_gemm_fp8.restype = ctypes.c_int
     lib.b200dq_gemm_fp8.argtypes = [ctypes.POINTER(Fp8GemmArgs), vp]
+    lib.b200dq_fp8_gated_fuses.restype = ctypes.c_int
+    lib.b200dq_fp8_gated_fuses.argtypes = [i32, i32, i32, i32]
     lib.b200dq_exchange_scratch_bytes.restype = sz
     lib.b200dq_exchange_scratch_bytes.argtypes = [i64, i32, i32]
     lib.b200dq_exchange_dispatch.restype = ctypes.c_int

@@ -534,7 +534,9 @@ int encode_fp8_map(CUtensorMap* map, const void* base, int rank, const cuuint64_
 }
 
 int check_fp8_gemm(const b200dq_fp8_gemm_args* a) {
-  if (a->a == nullptr || a->a_scale == nullptr || a->w == nullptr || a->w_scale == nullptr || a->c == nullptr)
+  const bool gated = a->gate_codes != nullptr;
+  if (a->a == nullptr || a->a_scale == nullptr || a->w == nullptr || a->w_scale == nullptr || (a->c == nullptr && !gated) ||
+      (gated && a->gate_scales == nullptr))
     return fail("gemm_fp8: null pointer");
   if (a->M <= 0 || a->N <= 0 || a->K <= 0) return fail("gemm_fp8: M, N, K must be positive (got %d, %d, %d)", a->M, a->N, a->K);
   if (a->num_groups < 0 || a->num_groups > 65535) return fail("gemm_fp8: num_groups=%d outside [0, 65535]", a->num_groups);
@@ -558,6 +560,14 @@ int check_fp8_gemm(const b200dq_fp8_gemm_args* a) {
   if (a->token_tile == 256 && a->num_groups > kFp8PairMaxGroups)
     return fail("gemm_fp8: the 256-token tile takes at most %d groups", kFp8PairMaxGroups);
   if (a->token_tile == 256 && a->split > 1) return fail("gemm_fp8: the 256-token tile does not split the contraction");
+  if (gated) {
+    if (a->trans_w || a->N % 256 != 0) return fail("gemm_fp8: a gated product needs gate and up rows in multiples of 128 (N=%d) and no trans_w", a->N);
+    if (a->out_type != OUT_BF16) return fail("gemm_fp8: the sums of a gated product are kept in bf16");
+    if (a->ld_gate < a->N / 2 || a->ld_gate % 16 != 0 || (reinterpret_cast<uintptr_t>(a->gate_codes) & 15) != 0)
+      return fail("gemm_fp8: rows of the gated codes must start on 16-byte boundaries");
+    if (a->gate_type != FP8_E4M3 && a->gate_type != FP8_E5M2) return fail("gemm_fp8: gated codes must be e4m3 or e5m2");
+    if (a->token_tile != 0 && a->token_tile != 256) return fail("gemm_fp8: a gated product takes the 256-token tile only");
+  }
   if (a->split < 0 || a->split > 8) return fail("gemm_fp8: split must be 0 to 8 (got %d)", a->split);
   return 0;
 }
@@ -587,7 +597,8 @@ int run_gemm_fp8(const b200dq_fp8_gemm_args* a, const DeviceState* ds, cudaStrea
   p.counts_int64 = a->counts_int64;
   p.num_groups = a->num_groups;
   p.status = ds->status;
-  const Fp8Plan plan = plan_fp8(a->M, a->num_groups, p.p_tiles, p.q_blocks, ds->sm_count, a->token_tile, a->split);
+  const bool gated = a->gate_codes != nullptr;
+  const Fp8Plan plan = plan_fp8(a->M, a->num_groups, p.p_tiles, p.q_blocks, ds->sm_count, gated ? 256 : a->token_tile, a->split);
   p.split = plan.split;
   CUtensorMap tmap_a, tmap_w;
   const cuuint64_t a_dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(a->M)};
@@ -600,6 +611,11 @@ int run_gemm_fp8(const b200dq_fp8_gemm_args* a, const DeviceState* ds, cudaStrea
   if (encode_fp8_map(&tmap_w, a->w, 3, w_dims, w_strides, kFp8BoxRows) != 0) return -1;
   if (plan.token_tile == 256) {
     p.p_tiles = (p.p_tiles + 1) / 2;
+    p.tile_cols = gated ? 128 : 256;
+    p.gate_codes = static_cast<uint8_t*>(a->gate_codes);
+    p.gate_scales = a->gate_scales;
+    p.ld_gate = a->ld_gate;
+    p.gate_fp8 = a->gate_type;
     CUDA_OK(launch_fp8_pair_gemm(tmap_a, tmap_w, p, static_cast<int>(std::min<long long>(plan.tiles, ds->sm_count / 2)), stream));
     return 0;
   }
@@ -986,6 +1002,11 @@ int b200dq_gemm_fp8(const b200dq_fp8_gemm_args* a, void* cuda_stream) {
   DeviceState* ds = nullptr;
   if (current_device_state(&ds) != 0) return -1;
   return run_gemm_fp8(a, ds, static_cast<cudaStream_t>(cuda_stream));
+}
+
+int b200dq_fp8_gated_fuses(int32_t M, int32_t N, int32_t K, int32_t num_groups) {
+  if (M <= 0 || N <= 0 || K <= 0 || N % 256 != 0 || num_groups < 0) return 0;
+  return plan_fp8(M, num_groups, N / 128, (K + 127) / 128, sm_count_or_bound(), 0, 0).token_tile == 256 ? 1 : 0;
 }
 
 size_t b200dq_exchange_scratch_bytes(int64_t tokens, int32_t top_k, int32_t num_experts) {

@@ -143,7 +143,7 @@ fp8_tile_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(fp8_smem_raw) + 1023) & ~uintptr_t(1023));
   float* scale_ring = reinterpret_cast<float*>(smem + C::kStages * C::kStageBytes);
   auto* ctl = reinterpret_cast<Fp8TileCtl<TN>*>(smem + C::kStages * C::kStageBytes + C::kScaleSlots * TN * 4);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int* abort_flag = &ctl->abort_flag;
   DeviceStatus* st = p.status;
   const int rank = static_cast<int>(cluster_rank());
@@ -191,31 +191,31 @@ fp8_tile_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = TOK_LANE ? make_idesc_f8(p.a_fmt, p.w_fmt, 0, p.trans_w, 128, 128)
-                                      : make_idesc_f8(p.w_fmt, p.a_fmt, p.trans_w, 0, 128, TN);
-      // the next 32 of the contraction: 32 bytes on in a row, or 32 rows on where rows run along it
-      const uint64_t w_step = p.trans_w ? 32 * 128 / 16 : 2;
-      uint32_t s = 0, phase = 0, i = 0;
-      bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb, ++i) {
-        const uint32_t buf = i % C::kAcc;
-        ok &= mbar_wait(&ctl->acc_empty[buf], ((i / C::kAcc) & 1u) ^ 1u, abort_flag, st, 2);
-        ok &= mbar_wait(&ctl->full[s], phase, abort_flag, st, 3);
-        tc_fence_after_sync();
-        if (ok) {
-          const uint32_t stage = smem_u32(smem + s * C::kStageBytes);
-          const uint64_t w_desc = make_smem_desc_sw128(stage), t_desc = make_smem_desc_sw128(stage + 128 * 128);
+    // the whole warp runs this loop, so that operands sit in uniform registers; one lane issues
+    const uint32_t idesc = TOK_LANE ? make_idesc_f8(p.a_fmt, p.w_fmt, 0, p.trans_w, 128, 128)
+                                    : make_idesc_f8(p.w_fmt, p.a_fmt, p.trans_w, 0, 128, TN);
+    // the next 32 of the contraction: 32 bytes on in a row, or 32 rows on where rows run along it
+    const uint64_t w_step = p.trans_w ? 32 * 128 / 16 : 2;
+    uint32_t s = 0, phase = 0, i = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb, ++i) {
+      const uint32_t buf = i % C::kAcc;
+      const uint32_t stage = smem_u32(smem + s * C::kStageBytes);
+      const uint64_t w_desc = make_smem_desc_sw128(stage), t_desc = make_smem_desc_sw128(stage + 128 * 128);
+      ok = ok && mbar_wait(&ctl->full[s], phase, abort_flag, st, 3);
+      ok = ok && mbar_wait(&ctl->acc_empty[buf], ((i / C::kAcc) & 1u) ^ 1u, abort_flag, st, 2);
+      tc_fence_after_sync();
+      if (ok && elect_one()) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint64_t w = w_desc + j * w_step, t = t_desc + 2 * j;
-            umma_ss_f8(tmem_base + buf * TN, TOK_LANE ? t : w, TOK_LANE ? w : t, idesc, j != 0);
-          }
+        for (int j = 0; j < 4; ++j) {
+          const uint64_t w = w_desc + j * w_step, t = t_desc + 2 * j;
+          umma_ss_f8(tmem_base + buf * TN, TOK_LANE ? t : w, TOK_LANE ? w : t, idesc, j != 0);
         }
-        tc_commit(&ctl->empty[s]);
         tc_commit(&ctl->acc_full[buf]);
-        if (++s == C::kStages) { s = 0; phase ^= 1u; }
+        tc_commit(&ctl->empty[s]);
       }
+      __syncwarp();
+      if (++s == C::kStages) { s = 0; phase ^= 1u; }
     }
   } else if (warp == 2) {
     if (!TOK_LANE) {

@@ -57,17 +57,19 @@ cudaError_t launch_fp8_tile_gemm(const CUtensorMap& tmap_a, const CUtensorMap& t
 cudaError_t launch_fp8_pair_gemm(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const Fp8GemmParams& p, int pairs,
                                  cudaStream_t stream) {
   static_assert(kFp8PairMaxGroups == kPairMaxGroups, "tile table");
-  static bool attr_set[kMaxDevices] = {};
+  static bool attr_set[kMaxDevices][2] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
-  if (!attr_set[dev]) {
-    e = cudaFuncSetAttribute(fp8_pair_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes);
+  const bool gated = p.gate_codes != nullptr;
+  auto kernel = gated ? fp8_pair_gemm_kernel<true> : fp8_pair_gemm_kernel<false>;
+  if (!attr_set[dev][gated]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes);
     if (e != cudaSuccess) return e;
-    attr_set[dev] = true;
+    attr_set[dev][gated] = true;
   }
-  fp8_pair_gemm_kernel<<<2 * pairs, kPairThreads, kPairSmemBytes, stream>>>(tmap_a, tmap_w, p);
+  kernel<<<2 * pairs, kPairThreads, kPairSmemBytes, stream>>>(tmap_a, tmap_w, p);
   return cudaGetLastError();
 }
 

@@ -26,6 +26,12 @@ struct Fp8GemmParams {
   int c_vec16;               // 16 bytes may be stored at once
   const void* counts;        // grouped: rows of each group, on the device; null: one group of M rows
   int counts_int64, num_groups;
+  // CTA pairs only
+  int tile_cols;             // columns of C that a tile advances by: 256, gated 128
+  uint8_t* gate_codes;       // gated: codes of silu(g) u, (M, P / 2), row pitch ld_gate; else null
+  float* gate_scales;        // (M, P / 256), contiguous
+  long long ld_gate;
+  int gate_fp8;
   int split;                 // CTAs of a cluster that share a tile's contraction
   DeviceStatus* status;
 };
@@ -37,7 +43,8 @@ constexpr int kFp8BoxRows = 128;    // rows of a weight box, and of a token box 
 cudaError_t launch_fp8_tile_gemm(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const Fp8GemmParams& p,
                                  bool tokens_on_lanes, int tile_tokens, long long tiles, cudaStream_t stream);
 
-// CTA pairs, 256 tokens x 256 columns (p.p_tiles counts tiles of 256); `pairs` clusters of two.
+// CTA pairs, 256 tokens x 256 columns (p.p_tiles counts tiles of p.tile_cols); `pairs` clusters of two. With
+// gate_codes the columns of a tile are 128 of the gate's and 128 of the up half's, and c (bf16) may be null.
 cudaError_t launch_fp8_pair_gemm(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const Fp8GemmParams& p, int pairs,
                                  cudaStream_t stream);
 constexpr int kFp8PairMaxGroups = 256;

@@ -1,19 +1,32 @@
 // The product of fp8_gemm.cuh for many tokens: CTA pairs, tiles of 256 tokens x 256 weight rows.
 //
 // A pair of CTAs on two SMs works on one tile with tcgen05.mma.cta_group::2 (M = N = 256): each CTA
-// loads 128 tokens and 128 weight rows per block of 128, 32 KB for 8.4 million multiply-adds, half of
-// what a CTA on its own would pull through L2 for the same work (at 128 x 256 the crossbar would
-// carry 14 TB/s at the tensor cores' rate). Its 128 x 256 sums per block go to one of two accumulators that
-// fill tensor memory, and eight warps move them, scaled, to fp32 registers: thread = one token, 128
-// columns, one scale per block. 64 packed fmas a thread and block are 256 cycles of the fp32 pipe,
-// and reading tensor memory about as many, under 512 cycles of multiplication.
+// loads 128 tokens and 128 weight rows per block of 128, 32 KB for 8.4 million multiply-adds, two thirds
+// of what a 128 x 256 tile of its own would pull through L2 for the same work. Its 128 x 256 sums per block go to
+// one of two accumulators that fill tensor memory, and eight warps move them, scaled, to fp32
+// registers: thread = one token, 128 columns, one scale per block; 64 packed fmas.
 //
-// Persistent: one pair per two SMs, tiles in strips of eight token tiles so that the tiles in flight
+// What bounds it (4096 x 28672 x 8192, 826 us, 2330 TFLOP/s, the GPU at its power limit near 1.55 GHz): the
+// hand-over of accumulators. With the summing warps reduced to the barriers alone it takes 695 us, without
+// waiting for them 618 us. Two accumulators are all that tensor memory holds at this width; four of
+// 128 columns (twice the instructions, each half as wide) measured 932 us. So everything on the way round
+// is short: the issuing warp runs uniformly (operands in uniform registers; a single issuing thread took
+// 920 us), commits the accumulator before the stage, and the summing warps hand back after
+// half of their additions. Strips of 16 token tiles: 826 us, 8: 840, 4: 868.
+//
+// Persistent: one pair per two SMs, tiles in strips of 16 token tiles so that the tiles in flight
 // share their operands in L2. warp 0: TMA producer (both CTAs); warp 1: MMA issuer (first CTA);
 // warps 2, 3: tensor memory, tile table; warps 4-11: sums and output. Finished rows go through 4 KB of
 // shared memory per warp, so that a store instruction writes whole 128-byte pieces.
+//
+// GATED: weights are [gate; up], F rows each; the first CTA loads 128 gate rows, the second the 128 up
+// rows that belong to them, so that a tile's columns 0-127 and 128-255 are g and u of the same 128
+// features: exactly one quantiser block. The two warps that hold a token's g and u swap a half each
+// through shared memory, compute silu(g) u on 64 columns each, agree on the maximum and write codes: h
+// (4 bytes per value out, 4 back in, or 2 and 2) never goes to memory unless the caller wants it.
 #pragma once
 #include "fp8_gemm.cuh"
+#include "fp8_quant.cuh"
 
 namespace b200dq {
 
@@ -22,7 +35,7 @@ constexpr int kPairStages = 6;
 constexpr int kPairHalf = 128 * 128;                          // one operand's half tile: 128 rows x 128 bytes
 constexpr int kPairStageBytes = 2 * kPairHalf;
 constexpr int kPairStageOut = 32 * 128;                       // a warp's output rows, 128 bytes each
-constexpr int kPairStrip = 8;
+constexpr int kPairStrip = 16;
 constexpr int kPairMaxGroups = 256;                           // groups whose tile table fits the control block
 // setmaxnreg moves registers from warps 0-3 to the eight summing warps: 128 * 40 + 256 * 232 = 384 * 168
 constexpr int kPairOtherRegs = 40, kPairSumRegs = 232;
@@ -80,7 +93,7 @@ __device__ __forceinline__ Fp8Tile fp8_pair_tile(const Fp8GemmParams& p, const F
   const int in_strip = static_cast<int>(t - strip * strip_tiles);
   const int high = min(kPairStrip, token_tiles - strip * kPairStrip);
   const int tt = strip * kPairStrip + in_strip % high;
-  const int p0 = in_strip / high * 256;
+  const int p0 = in_strip / high * p.tile_cols;
   if (p.counts == nullptr) return Fp8Tile{0, tt * 256, p.M, p0};
   int lo = 0, hi = p.num_groups;                              // tile_prefix[lo] <= tt < tile_prefix[hi]
   while (hi - lo > 1) {
@@ -142,6 +155,74 @@ __device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, uint8_t* 
   }
 }
 
+// acc[at ..] += scale * 32 columns, in pairs.
+__device__ __forceinline__ void fp8_pair_add(uint64_t (&acc)[64], const int at, const uint32_t (&v)[32], uint64_t scale) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) acc[at + j] = ffma2(pack2(v[2 * j], v[2 * j + 1]), scale, acc[at + j]);
+}
+
+// silu(g) * u with the hardware's exponential and reciprocal: a relative error near 2^-21, far below the
+// codes' half step of 2^-4 or 2^-3. For g so low that e^-g is infinite the reciprocal is zero.
+__device__ __forceinline__ float fast_silu_mul(float g, float u) { return g * __fdividef(1.0f, 1.0f + __expf(-g)) * u; }
+
+__device__ __forceinline__ void pair_barrier(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+
+// The two warps of a lane quarter: `half` 0 holds g, 1 holds u of 32 tokens x 128 features. Each sends
+// the half that the other one works on (32 columns at a time, 16-byte chunks rotated by the row), then
+// quantises its 64 features. `mine`, `other`: their 4 KB of shared memory.
+template <int FP8>
+__device__ __forceinline__ void fp8_pair_gate(const Fp8GemmParams& p, uint8_t* mine, const uint8_t* other, const uint64_t (&acc)[64],
+                                              int half, int quarter, long long m, bool in, int f0, int lane) {
+  float act[64];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    // half 0 keeps columns 0-63 and sends 64-127, half 1 the other way round
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint64_t lo = half == 0 ? acc[32 + r * 16 + 2 * j] : acc[r * 16 + 2 * j];
+      const uint64_t hi = half == 0 ? acc[32 + r * 16 + 2 * j + 1] : acc[r * 16 + 2 * j + 1];
+      const float2 a = unpack2(lo), b = unpack2(hi);
+      *reinterpret_cast<float4*>(mine + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(a.x, a.y, b.x, b.y);
+    }
+    pair_barrier(1 + quarter);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float4 o = *reinterpret_cast<const float4*>(other + lane * 128 + ((j ^ (lane & 7)) << 4));
+      const float2 a = unpack2(half == 0 ? acc[r * 16 + 2 * j] : acc[32 + r * 16 + 2 * j]);
+      const float2 b = unpack2(half == 0 ? acc[r * 16 + 2 * j + 1] : acc[32 + r * 16 + 2 * j + 1]);
+      const float own[4] = {a.x, a.y, b.x, b.y}, got[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        act[r * 32 + 4 * j + e] = half == 0 ? fast_silu_mul(own[e], got[e]) : fast_silu_mul(got[e], own[e]);
+    }
+    pair_barrier(1 + quarter);
+  }
+  uint32_t m_bits = 0;
+#pragma unroll
+  for (int j = 0; j < 64; ++j) m_bits = max(m_bits, magnitude_bits(act[j]));
+  reinterpret_cast<uint32_t*>(mine)[lane] = m_bits;
+  pair_barrier(1 + quarter);
+  m_bits = max(m_bits, reinterpret_cast<const uint32_t*>(other)[lane]);
+  pair_barrier(1 + quarter);                                  // read before the next tile's rows overwrite it
+  const float s = fp8_scale_of<FP8>(m_bits);
+  const float inv = __frcp_rn(s);
+  if (in) {
+    uint8_t* dst = p.gate_codes + m * p.ld_gate + f0 + half * 64;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float* a = act + j * 16 + i * 4;
+        w[i] = fp8_pair<FP8>(__fmul_rn(a[0], inv), __fmul_rn(a[1], inv)) | (fp8_pair<FP8>(__fmul_rn(a[2], inv), __fmul_rn(a[3], inv)) << 16);
+      }
+      *reinterpret_cast<uint4*>(dst + j * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (half == 0) p.gate_scales[m * p.p_tiles + f0 / 128] = s;
+  }
+}
+
+template <bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                      const Fp8GemmParams p) {
@@ -149,7 +230,7 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   uint8_t* smem = fp8_pair_smem;
   uint8_t* stage_out = smem + kPairStages * kPairStageBytes;
   auto* ctl = reinterpret_cast<Fp8PairCtl*>(stage_out + 8 * kPairStageOut);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int* abort_flag = &ctl->abort_flag;
   DeviceStatus* st = p.status;
   const int rank = static_cast<int>(cluster_rank());
@@ -184,9 +265,9 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       bool ok = true;
       for (long long t = pair; ok && t < tiles; t += pairs) {
         const Fp8Tile tile = fp8_pair_tile(p, ctl, token_tiles, t);
-        const int m0 = tile.m0 + rank * 128, p0 = tile.p0 + rank * 128;
+        const int m0 = tile.m0 + rank * 128, p0 = tile.p0 + rank * (GATED ? p.P / 2 : 128);
         for (int kb = 0; kb < p.q_blocks; ++kb) {
-          ok = mbar_wait_cluster(&ctl->empty[s], phase ^ 1u, abort_flag, st, 11);
+          ok = mbar_wait(&ctl->empty[s], phase ^ 1u, abort_flag, st, 11);
           if (!ok) break;
           uint8_t* stage = smem + s * kPairStageBytes;
           const uint32_t bar = cluster_map(smem_u32(&ctl->full[s]), 0);
@@ -197,7 +278,7 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
           if (++s == kPairStages) { s = 0; phase ^= 1u; }
         }
       }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+    } else if (warp == 1 && rank == 0) {
       // ---------------- MMA issuer for both CTAs ----------------
       const uint32_t idesc = make_idesc_f8(p.a_fmt, p.w_fmt, 0, p.trans_w, 256, 256);
       const uint64_t w_step = p.trans_w ? 32 * 128 / 16 : 2;
@@ -205,19 +286,20 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       bool ok = true;
       for (long long t = pair; t < tiles; t += pairs) {
         for (int kb = 0; kb < p.q_blocks; ++kb, ++i) {
-          const uint32_t buf = i & 1u;
-          ok = ok && mbar_wait_cluster(&ctl->acc_empty[buf], ((i >> 1) & 1u) ^ 1u, abort_flag, st, 12);
-          ok = ok && mbar_wait_cluster(&ctl->full[s], phase, abort_flag, st, 13);
+          const uint32_t buf = i & 1u, acc = tmem_base + buf * 256;
+          const uint32_t stage = smem_u32(smem + s * kPairStageBytes);
+          const uint64_t a_desc = make_smem_desc_sw128(stage), w_desc = make_smem_desc_sw128(stage + kPairHalf);
+          ok = ok && mbar_wait(&ctl->full[s], phase, abort_flag, st, 13);
+          ok = ok && mbar_wait(&ctl->acc_empty[buf], ((i >> 1) & 1u) ^ 1u, abort_flag, st, 12);
           tc_fence_after_sync();
-          if (ok) {
-            const uint32_t stage = smem_u32(smem + s * kPairStageBytes);
-            const uint64_t a_desc = make_smem_desc_sw128(stage), w_desc = make_smem_desc_sw128(stage + kPairHalf);
+          if (ok && elect_one()) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              umma_pair_ss_f8(tmem_base + buf * 256, a_desc + 2 * j, w_desc + j * w_step, idesc, j != 0);
+              umma_pair_ss_f8(acc, a_desc + 2 * j, w_desc + j * w_step, idesc, j != 0);
+            tc_commit_pair(&ctl->acc_full[buf]);
+            tc_commit_pair(&ctl->empty[s]);
           }
-          tc_commit_pair(&ctl->empty[s]);
-          tc_commit_pair(&ctl->acc_full[buf]);
+          __syncwarp();
           if (++s == kPairStages) { s = 0; phase ^= 1u; }
         }
       }
@@ -228,50 +310,77 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     uint8_t* stage = stage_out + (warp - 4) * kPairStageOut;
-    uint32_t empty_bar[2];
-    for (int b = 0; b < 2; ++b) empty_bar[b] = cluster_map(smem_u32(&ctl->acc_empty[b]), 0);
+    const uint32_t empty_bar = cluster_map(smem_u32(&ctl->acc_empty[0]), 0);
+    const uint32_t acc_addr = tmem_base + lane_addr + half * 128;
     uint32_t i = 0;
     bool ok = true;
     for (long long t = pair; t < tiles; t += pairs) {
       const Fp8Tile tile = fp8_pair_tile(p, ctl, token_tiles, t);
       const int m_first = tile.m0 + rank * 128 + quarter * 32;
-      const int p_block = min(tile.p0 / 128 + half, (p.P - 1) / 128);       // a tile may end before its second half
+      // a tile may end before its second half; gated, the second half is the up half of the weight
+      const int p_block = GATED ? (tile.p0 + half * (p.P / 2)) / 128 : min(tile.p0 / 128 + half, (p.P - 1) / 128);
       const float* as = p.a_scale + static_cast<long long>(min(m_first + lane, p.M - 1)) * p.ld_a_scale;
       const float* ws = p.w_scale + tile.group * p.ws_group + p_block * p.ws_p;
       uint64_t acc[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) acc[j] = 0;
       // the scales two blocks ahead: their latency is longer than a block's multiplication
-      float s0 = as[0] * ws[0], s1 = p.q_blocks > 1 ? as[1] * ws[p.ws_q] : 0.f;
+      float a0 = as[0], w0 = ws[0], a1 = 0.f, w1 = 0.f;
+      if (p.q_blocks > 1) { a1 = as[1]; w1 = ws[p.ws_q]; }
+      as += 2; ws += 2 * p.ws_q;
+      // Two pieces of 32 columns are in registers or on their way at any time; the order hands the accumulator
+      // back after half of the additions and fetches the next block's first half under the other half.
+      uint32_t v[2][32];
+      ok &= mbar_wait(&ctl->acc_full[i & 1u], (i >> 1) & 1u, abort_flag, st, 14);
+      __syncwarp();
+      tc_fence_after_sync();
+      tmem_ld_32x32b_x32(acc_addr + (i & 1u) * 256, v[0]);
+      tmem_ld_32x32b_x32(acc_addr + (i & 1u) * 256 + 32, v[1]);
+#pragma unroll 1
       for (int kb = 0; kb < p.q_blocks; ++kb, ++i) {
-        const uint32_t buf = i & 1u;
+        const uint32_t buf = i & 1u, addr = acc_addr + buf * 256, next = acc_addr + (buf ^ 1u) * 256;
+        const bool more = kb + 1 < p.q_blocks;
         float a2 = 0.f, w2 = 0.f;
-        if (kb + 2 < p.q_blocks) { a2 = as[kb + 2]; w2 = ws[(kb + 2) * p.ws_q]; }
-        const uint64_t scale = pack2f(s0, s0);
-        ok &= mbar_wait_warp(&ctl->acc_full[buf], (i >> 1) & 1u, abort_flag, st, 14, lane);
-        tc_fence_after_sync();
-        const uint32_t addr = tmem_base + lane_addr + buf * 256 + half * 128;
-        uint32_t v[2][32];
-        tmem_ld_32x32b_x32(addr, v[0]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tc_wait_ld(v[c & 1]);
-          if (c < 3) tmem_ld_32x32b_x32(addr + (c + 1) * 32, v[(c + 1) & 1]);
-          if (c == 3) {
-            // the accumulator goes back before the last additions
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(empty_bar[buf]);
-          }
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            acc[c * 16 + j] = ffma2(pack2(v[c & 1][2 * j], v[c & 1][2 * j + 1]), scale, acc[c * 16 + j]);
+        if (kb + 2 < p.q_blocks) {
+          a2 = *as; w2 = *ws;
+          ++as; ws += p.ws_q;
         }
-        s0 = s1;
-        s1 = a2 * w2;
+        const float s0 = a0 * w0;
+        const uint64_t scale = pack2f(s0, s0);
+        tc_wait_ld(v[0]);
+        tc_wait_ld(v[1]);
+        fp8_pair_add(acc, 0, v[0], scale);
+        tmem_ld_32x32b_x32(addr + 64, v[0]);
+        fp8_pair_add(acc, 16, v[1], scale);
+        tmem_ld_32x32b_x32(addr + 96, v[1]);
+        tc_wait_ld(v[0]);
+        tc_wait_ld(v[1]);
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(empty_bar + 8 * buf);
+        fp8_pair_add(acc, 32, v[0], scale);
+        if (more) {
+          ok &= mbar_wait(&ctl->acc_full[buf ^ 1u], ((i + 1) >> 1) & 1u, abort_flag, st, 14);
+          __syncwarp();
+          tc_fence_after_sync();
+          tmem_ld_32x32b_x32(next, v[0]);
+        }
+        fp8_pair_add(acc, 48, v[1], scale);
+        if (more) tmem_ld_32x32b_x32(next + 32, v[1]);
+        a0 = a1; w0 = w1; a1 = a2; w1 = w2;
       }
-      if (ok) {
-        const int rows = min(32, tile.m_end - m_first);
+      const int rows = min(32, tile.m_end - m_first);
+      if (GATED) {
+        // both warps of a quarter meet in here, whatever happened to either
+        const uint8_t* other = stage_out + ((warp - 4) ^ 4) * kPairStageOut;
+        const bool in = ok && lane < rows;
+        if (p.gate_fp8 == FP8_E4M3)
+          fp8_pair_gate<FP8_E4M3>(p, stage, other, acc, half, quarter, m_first + lane, in, tile.p0, lane);
+        else
+          fp8_pair_gate<FP8_E5M2>(p, stage, other, acc, half, quarter, m_first + lane, in, tile.p0, lane);
+        if (ok && p.c != nullptr)
+          fp8_pair_store<OUT_BF16>(p, stage, acc, m_first, rows, tile.p0 + half * (p.P / 2), lane);
+      } else if (ok) {
         const int col0 = tile.p0 + half * 128;
         if (p.out_type == OUT_BF16) fp8_pair_store<OUT_BF16>(p, stage, acc, m_first, rows, col0, lane);
         else if (p.out_type == OUT_F16) fp8_pair_store<OUT_F16>(p, stage, acc, m_first, rows, col0, lane);

@@ -852,12 +852,26 @@ def gemm_fp8_gated(a: torch.Tensor, a_scale: torch.Tensor, w: Fp8Weight, counts=
     _check_fp8_target(dtype)
     if w.N % 2:
         raise ValueError("w must have an even number of rows: gate above up")
-    if counts is None:
-        h = gemm_fp8(a, a_scale, w, out_dtype=torch.float32)
-    else:
-        h = gemm_fp8_grouped(a, a_scale, w, counts, out_dtype=torch.float32)
-    codes, scales = silu_mul_quant_fp8(h, dtype)
-    return (codes, scales, h.to(torch.bfloat16)) if keep_h else (codes, scales)
+    lib = _lib.load()
+    args = _fp8_gemm_args("gemm_fp8_gated", a, a_scale, w, False, grouped=counts is not None)
+    M, F, dev = a.shape[0], w.N // 2, a.device
+    if counts is not None:
+        counts = _device_counts(counts, w.num_groups, M, dev)
+        args.counts, args.counts_int64 = counts.data_ptr(), 1 if counts.dtype == torch.int64 else 0
+    _ensure_init(dev)
+    if not lib.b200dq_fp8_gated_fuses(M, w.N, w.K, w.num_groups):
+        h = _run_gemm_fp8(args, torch.empty((M, w.N), dtype=torch.float32, device=dev), "b200dq_gemm_fp8")
+        codes, scales = silu_mul_quant_fp8(h, dtype)
+        return (codes, scales, h.to(torch.bfloat16)) if keep_h else (codes, scales)
+    codes = _fp8_rows(M, F, dtype, dev)
+    scales = torch.empty((M, _blocks128(F)), dtype=torch.float32, device=dev)
+    h = torch.empty((M, w.N), dtype=torch.bfloat16, device=dev) if keep_h else None
+    args.c, args.out_type = h.data_ptr() if keep_h else None, _lib.OUT_BF16
+    args.gate_codes, args.gate_scales, args.ld_gate = codes.data_ptr(), scales.data_ptr(), codes.stride(0)
+    args.gate_type = _FP8_OF[dtype]
+    with torch.cuda.device(dev):
+        _lib.check(lib.b200dq_gemm_fp8(ctypes.byref(args), _stream_ptr(dev)), "b200dq_gemm_fp8 (gated)")
+    return (codes, scales, h) if keep_h else (codes, scales)
 
 
 def check_status(device: Optional[torch.device] = None) -> None:
