@@ -27,6 +27,8 @@ import torch
 import torch.distributed as dist
 from torch.autograd.function import once_differentiable
 
+from . import _lib, ops
+
 
 def route(logits: torch.Tensor, top_k: int):
     scores = torch.softmax(logits.float(), dim=-1)
@@ -90,7 +92,6 @@ def make_gpu_expert_mlp(w1_packed, w2_packed, token_tile: Optional[int] = None) 
     """The expert MLP on this library's kernels. ``token_tile=None`` picks the tile per call
     (:func:`expert_token_tile`): on the 64-expert, top-6 layer with 16384 tokens the 128-token tile
     measured 2.49 ms against 3.19 ms for the 256-token tile."""
-    from . import ops
 
     def gemm(w):
         def run(x, counts):
@@ -128,7 +129,6 @@ class ExchangePlan:
 
 
 def _check_experts(x: torch.Tensor, experts: torch.Tensor, num_experts: int) -> torch.Tensor:
-    from . import ops
     ops._check_rows("x", x)
     if x.dtype not in ops._FLOAT_OF:
         raise TypeError(f"x must be float16, bfloat16 or float32, got {x.dtype}")
@@ -148,7 +148,6 @@ def _check_experts(x: torch.Tensor, experts: torch.Tensor, num_experts: int) -> 
 def _exchange_out(x: torch.Tensor, experts: torch.Tensor, num_experts: int, out: torch.Tensor,
                   scales: Optional[torch.Tensor], dtype: Optional[torch.dtype]) -> ExchangePlan:
     """Sorts the pairs and moves the rows of ``x`` into ``out``, on the current stream."""
-    from . import _lib, ops
     lib = _lib.load()
     T, k = experts.shape
     plan = ExchangePlan(torch.empty((T, k), dtype=torch.int64, device=x.device),
@@ -156,18 +155,15 @@ def _exchange_out(x: torch.Tensor, experts: torch.Tensor, num_experts: int, out:
     if T == 0:
         plan.counts.zero_()
         return plan
-    ops._ensure_init(x.device)
     need = lib.b200dq_exchange_scratch_bytes(T, k, num_experts)
     # scratch of this call alone: calls on two streams, or in two graphs, share nothing
     scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    with torch.cuda.device(x.device):
-        _lib.check(lib.b200dq_exchange_dispatch(
-            experts.data_ptr(), 1 if experts.dtype == torch.int64 else 0, T, k, num_experts,
-            x.data_ptr(), x.stride(0) if T > 1 else x.shape[1], x.shape[1], ops._FLOAT_OF[x.dtype], out.data_ptr(),
-            out.stride(0) if out.shape[0] > 1 else max(out.stride(0), out.shape[1]),
-            scales.data_ptr() if scales is not None else None, ops._FP8_OF[dtype] if dtype is not None else 0,
-            plan.row_of.data_ptr(), plan.counts.data_ptr(), scratch.data_ptr() if need else None, need,
-            ops._stream_ptr(x.device)), "b200dq_exchange_dispatch")
+    width = x.shape[1]
+    ops._call(lib.b200dq_exchange_dispatch, "b200dq_exchange_dispatch", x.device,
+              experts.data_ptr(), 1 if experts.dtype == torch.int64 else 0, T, k, num_experts,
+              x.data_ptr(), x.stride(0) if T > 1 else width, width, ops._FLOAT_OF[x.dtype], out.data_ptr(),
+              out.stride(0), scales.data_ptr() if scales is not None else None, ops._FP8_OF[dtype] if dtype is not None else 0,
+              plan.row_of.data_ptr(), plan.counts.data_ptr(), scratch.data_ptr() if need else None, need)
     return plan
 
 
@@ -190,15 +186,12 @@ class _Dispatch(torch.autograd.Function):
 
 
 def _exchange_sum(y: torch.Tensor, row_of: torch.Tensor, weights: Optional[torch.Tensor]) -> torch.Tensor:
-    from . import _lib, ops
     T, k = row_of.shape
     out = torch.empty((T, y.shape[1]), dtype=y.dtype, device=y.device)
     if T:
-        ops._ensure_init(y.device)
-        with torch.cuda.device(y.device):
-            _lib.check(_lib.load().b200dq_exchange_sum(
-                y.data_ptr(), row_of.data_ptr(), weights.data_ptr() if weights is not None else None, out.data_ptr(),
-                T, k, y.shape[1], ops._FLOAT_OF[y.dtype], ops._stream_ptr(y.device)), "b200dq_exchange_sum")
+        ops._call(_lib.load().b200dq_exchange_sum, "b200dq_exchange_sum", y.device, y.data_ptr(), row_of.data_ptr(),
+                  weights.data_ptr() if weights is not None else None, out.data_ptr(), T, k, y.shape[1],
+                  ops._FLOAT_OF[y.dtype])
     return out
 
 
@@ -211,18 +204,15 @@ class _Combine(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
-        from . import _lib, ops
         y, row_of, weights = ctx.saved_tensors
         T, k = row_of.shape
         d_out = d_out.contiguous()
         d_y = torch.empty_like(y) if ctx.needs_input_grad[0] else None
         d_w = torch.empty_like(weights) if ctx.needs_input_grad[2] else None
         if T:
-            with torch.cuda.device(y.device):
-                _lib.check(_lib.load().b200dq_exchange_sum_grad(
-                    d_out.data_ptr(), y.data_ptr(), row_of.data_ptr(), weights.data_ptr(),
-                    d_y.data_ptr() if d_y is not None else None, d_w.data_ptr() if d_w is not None else None,
-                    T, k, y.shape[1], ops._FLOAT_OF[y.dtype], ops._stream_ptr(y.device)), "b200dq_exchange_sum_grad")
+            ops._call(_lib.load().b200dq_exchange_sum_grad, "b200dq_exchange_sum_grad", y.device, d_out.data_ptr(),
+                      y.data_ptr(), row_of.data_ptr(), weights.data_ptr(), d_y.data_ptr() if d_y is not None else None,
+                      d_w.data_ptr() if d_w is not None else None, T, k, y.shape[1], ops._FLOAT_OF[y.dtype])
         return d_y, None, d_w
 
 
@@ -233,8 +223,11 @@ def dispatch(x: torch.Tensor, experts: torch.Tensor, num_experts: int) -> Tuple[
     whose id lies outside [0, num_experts) -- a padded token's, say -- takes part in nothing: it gets a row of
     zeros behind the last expert's. Differentiable in x (float32 sums over the slots, in their order)."""
     experts = _check_experts(x, experts, num_experts)
-    rows, row_of, counts = _Dispatch.apply(x, experts, num_experts)
-    return rows, ExchangePlan(row_of, counts)
+    if torch.is_grad_enabled() and x.requires_grad:
+        rows, row_of, counts = _Dispatch.apply(x, experts, num_experts)
+        return rows, ExchangePlan(row_of, counts)
+    rows = torch.empty((experts.numel(), x.shape[1]), dtype=x.dtype, device=x.device)
+    return rows, _exchange_out(x, experts, num_experts, rows, None, None)
 
 
 def dispatch_fp8(x: torch.Tensor, experts: torch.Tensor, num_experts: int,
@@ -242,7 +235,6 @@ def dispatch_fp8(x: torch.Tensor, experts: torch.Tensor, num_experts: int,
     """:func:`dispatch` with every token quantised once on its way, as :func:`ops.quant_fp8` does it: returns
     ``(codes (T * k, H), scales (T * k, ceil(H / 128)), plan)``. Not differentiable. A dropped pair's row has
     zero codes."""
-    from . import ops
     ops._check_fp8_target(dtype)
     experts = _check_experts(x, experts, num_experts)
     rows = experts.numel()
@@ -255,7 +247,6 @@ def combine(y: torch.Tensor, plan: ExchangePlan, weights: torch.Tensor) -> torch
     """Back from expert order: ``out[t] = sum_s weights[t, s] * y[plan.row_of[t, s]]``, float32 sums in slot order
     rounded once to y's dtype; dropped pairs add nothing. ``y`` (T * k, H) contiguous float16, bfloat16 or float32,
     ``weights`` (T, k) of any floating type. Differentiable in y and weights."""
-    from . import ops
     ops._check_cuda_contig("y", y)
     if y.dim() != 2 or y.dtype not in ops._FLOAT_OF:
         raise ValueError("y must be a 2-D float16, bfloat16 or float32 tensor")
@@ -266,7 +257,10 @@ def combine(y: torch.Tensor, plan: ExchangePlan, weights: torch.Tensor) -> torch
         raise ValueError(f"weights must be floating point of shape {tuple(row_of.shape)}, got {weights.dtype} {tuple(weights.shape)}")
     if y.shape[0] != row_of.numel() or y.shape[1] == 0:
         raise ValueError(f"y must have {row_of.numel()} rows of at least one column, got {tuple(y.shape)}")
-    return _Combine.apply(y, row_of, weights.float().contiguous())
+    weights = weights.float().contiguous()
+    if not torch.is_grad_enabled() or not (y.requires_grad or weights.requires_grad):
+        return _exchange_sum(y, row_of, weights)
+    return _Combine.apply(y, row_of, weights)
 
 
 def moe_forward(x: torch.Tensor, logits: torch.Tensor, top_k: int, num_experts: int, mlp: ExpertMLP) -> torch.Tensor:

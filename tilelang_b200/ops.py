@@ -592,6 +592,26 @@ _FP8_OF = {torch.float8_e4m3fn: _lib.FP8_E4M3, torch.float8_e5m2: _lib.FP8_E5M2}
 _FLOAT_OF = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
+def _call(fn, what: str, device: torch.device, *args) -> None:
+    """``fn(*args, stream)`` on the device's current stream. Decode steps are a few microseconds on the GPU,
+    so the device is switched only when it is not the current one (the context manager and a
+    ``torch.cuda.Stream`` object cost 10 us of 20 per call)."""
+    idx = device.index
+    if idx not in _initialised_devices:
+        _ensure_init(device)
+    if _current_device() == idx:
+        rc = fn(*args, _raw_stream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args, _raw_stream(idx))
+    if rc:
+        _lib.check(rc, what)
+
+
 def _blocks128(n: int) -> int:
     return (n + 127) // 128
 
@@ -616,6 +636,8 @@ def _check_rows(name: str, t: torch.Tensor, device: Optional[torch.device] = Non
 
 def _fp8_rows(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
     """(rows, cols) codes whose row pitch is a multiple of 16 bytes, as the products read them."""
+    if cols % 16 == 0:
+        return torch.empty((rows, cols), dtype=dtype, device=device)
     return torch.empty((rows, (cols + 15) // 16 * 16), dtype=dtype, device=device)[:, :cols]
 
 
@@ -645,11 +667,8 @@ def _quant_fp8(mode: int, what: str, x: torch.Tensor, d: Optional[torch.Tensor],
     codes = _fp8_rows(rows, out_cols, dtype, x.device)
     scales = torch.empty((rows, _blocks128(out_cols)), dtype=torch.float32, device=x.device)
     if rows:
-        _ensure_init(x.device)
-        with torch.cuda.device(x.device):
-            _lib.check(lib.b200dq_quant_fp8(mode, x.data_ptr(), ld_x, d.data_ptr() if d is not None else None, ld_d,
-                                            codes.data_ptr(), codes.stride(0), scales.data_ptr(), rows, cols,
-                                            _FLOAT_OF[x.dtype], _FP8_OF[dtype], _stream_ptr(x.device)), what)
+        _call(lib.b200dq_quant_fp8, what, x.device, mode, x.data_ptr(), ld_x, d.data_ptr() if d is not None else None,
+              ld_d, codes.data_ptr(), codes.stride(0), scales.data_ptr(), rows, cols, _FLOAT_OF[x.dtype], _FP8_OF[dtype])
     return codes, scales
 
 
@@ -720,11 +739,8 @@ def quant_fp8_weight(w: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) 
     lead, (N, K) = w.shape[:-2], w.shape[-2:]
     codes = torch.empty((*lead, N, (K + 15) // 16 * 16), dtype=dtype, device=w.device)[..., :K]
     scales = torch.empty((*lead, _blocks128(N), _blocks128(K)), dtype=torch.float32, device=w.device)
-    _ensure_init(w.device)
-    with torch.cuda.device(w.device):
-        _lib.check(lib.b200dq_quant_fp8_blocks(w.data_ptr(), codes.data_ptr(), codes.stride(-2), scales.data_ptr(),
-                                               w.shape[0] if lead else 1, N, K, _FLOAT_OF[w.dtype], _FP8_OF[dtype],
-                                               _stream_ptr(w.device)), "b200dq_quant_fp8_blocks")
+    _call(lib.b200dq_quant_fp8_blocks, "b200dq_quant_fp8_blocks", w.device, w.data_ptr(), codes.data_ptr(),
+          codes.stride(-2), scales.data_ptr(), w.shape[0] if lead else 1, N, K, _FLOAT_OF[w.dtype], _FP8_OF[dtype])
     return Fp8Weight(codes, scales)
 
 
@@ -769,10 +785,10 @@ def _fp8_gemm_args(what: str, a: torch.Tensor, a_scale: torch.Tensor, w: Fp8Weig
     ld_scale = _check_rows("a_scale", a_scale, dev)
     if a_scale.dtype != torch.float32 or tuple(a_scale.shape) != (M, _blocks128(inner)):
         raise ValueError(f"a_scale must be float32 of shape {(M, _blocks128(inner))}, got {a_scale.dtype} {tuple(a_scale.shape)}")
-    return _lib.Fp8GemmArgs(
-        a=a.data_ptr(), a_scale=a_scale.data_ptr(), w=codes.data_ptr(), w_scale=scales.data_ptr(),
-        lda=lda, ld_a_scale=ld_scale, ldw=ldw, w_group_stride=group_stride, M=M, N=N, K=K,
-        num_groups=G, a_type=_FP8_OF[a.dtype], w_type=_FP8_OF[codes.dtype], trans_w=1 if trans_w else 0)
+    # in the order of the struct: a, a_scale, w, w_scale, c, counts, pitches, sizes, groups, types
+    return _lib.Fp8GemmArgs(a.data_ptr(), a_scale.data_ptr(), codes.data_ptr(), scales.data_ptr(), None, None,
+                            lda, ld_scale, ldw, group_stride, M, N, K, G, 0, _FP8_OF[a.dtype], _FP8_OF[codes.dtype],
+                            0, 1 if trans_w else 0)
 
 
 def _fp8_gemm_out(M: int, cols: int, out: Optional[torch.Tensor], out_dtype: torch.dtype, device: torch.device):
@@ -789,11 +805,8 @@ def _fp8_gemm_out(M: int, cols: int, out: Optional[torch.Tensor], out_dtype: tor
 def _run_gemm_fp8(args, out: torch.Tensor, what: str) -> torch.Tensor:
     if args.M == 0:
         return out
-    lib = _lib.load()
     args.c, args.out_type = out.data_ptr(), _OUT_OF[out.dtype]
-    _ensure_init(out.device)
-    with torch.cuda.device(out.device):
-        _lib.check(lib.b200dq_gemm_fp8(ctypes.byref(args), _stream_ptr(out.device)), what)
+    _call(_lib.load().b200dq_gemm_fp8, what, out.device, ctypes.byref(args))
     return out
 
 
@@ -869,8 +882,7 @@ def gemm_fp8_gated(a: torch.Tensor, a_scale: torch.Tensor, w: Fp8Weight, counts=
     args.c, args.out_type = h.data_ptr() if keep_h else None, _lib.OUT_BF16
     args.gate_codes, args.gate_scales, args.ld_gate = codes.data_ptr(), scales.data_ptr(), codes.stride(0)
     args.gate_type = _FP8_OF[dtype]
-    with torch.cuda.device(dev):
-        _lib.check(lib.b200dq_gemm_fp8(ctypes.byref(args), _stream_ptr(dev)), "b200dq_gemm_fp8 (gated)")
+    _call(lib.b200dq_gemm_fp8, "b200dq_gemm_fp8 (gated)", dev, ctypes.byref(args))
     return (codes, scales, h) if keep_h else (codes, scales)
 
 
