@@ -49,18 +49,27 @@ __device__ __forceinline__ void warp_exclusive_scan(int* bins, int n, int lane) 
 // Rows of the pairs [first, last) in pair order, by one warp: next[e] is the next free row of expert e.
 __device__ __forceinline__ void warp_place(const ExchangeSortParams& p, long long first, long long last, int* next,
                                            int lane) {
-  for (long long base = first; base < last; base += 32) {
-    const long long i = base + lane;
-    const bool in = i < last;
-    const int e = in ? expert_of(p, i) : p.num_experts + 1;          // a bin of its own, never placed
-    const unsigned peers = __match_any_sync(0xffffffffu, e);
-    const int rank = __popc(peers & ((1u << lane) - 1u));
-    int row = 0;
-    if (in) row = next[e] + rank;
-    __syncwarp();
-    if (in && rank == 0) next[e] += __popc(peers);
-    __syncwarp();
-    if (in) p.row_of[i] = e == p.num_experts ? -1ll - row : static_cast<long long>(row);
+  for (long long base = first; base < last; base += 128) {
+    int ids[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const long long i = base + 32 * j + lane;
+      ids[j] = i < last ? expert_of(p, i) : p.num_experts + 1;       // a bin of its own, never placed
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const long long i = base + 32 * j + lane;
+      const bool in = i < last;
+      const int e = ids[j];
+      const unsigned peers = __match_any_sync(0xffffffffu, e);
+      const int rank = __popc(peers & ((1u << lane) - 1u));
+      int row = 0;
+      if (in) row = next[e] + rank;
+      __syncwarp();
+      if (in && rank == 0) next[e] += __popc(peers);
+      __syncwarp();
+      if (in) p.row_of[i] = e == p.num_experts ? -1ll - row : static_cast<long long>(row);
+    }
   }
 }
 
@@ -215,44 +224,40 @@ __global__ void __launch_bounds__(kPlaceWarps * 32) exchange_place_kernel(const 
   extern __shared__ int exchange_smem[];
   const int bins = p.num_experts + 1;
   int* all = exchange_smem;                // [bins]
-  int* next = exchange_smem + bins;        // [warps][bins]
+  int* before = exchange_smem + bins;      // [bins]
+  int* next = exchange_smem + 2 * bins;    // [warps][bins]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long first = blockIdx.x * per, last = min(p.tokens * p.top_k, first + per);
   const long long piece = ((per + kPlaceWarps - 1) / kPlaceWarps + 31) / 32 * 32;
   const long long w0 = min(last, first + warp * piece), w1 = min(last, w0 + piece);
-  for (int i = threadIdx.x; i < (kPlaceWarps + 1) * bins; i += kPlaceWarps * 32) exchange_smem[i] = 0;
+  for (int i = threadIdx.x; i < (kPlaceWarps + 2) * bins; i += kPlaceWarps * 32) exchange_smem[i] = 0;
   __syncthreads();
   for (long long i = w0 + lane; i < w1; i += 32) atomicAdd(&next[warp * bins + expert_of(p, i)], 1);
-  int before_of[(kExchangeMaxExperts + kPlaceWarps * 32) / (kPlaceWarps * 32)];
+  // a warp adds up every eighth chunk's counts, its lanes neighbouring experts
+  for (int e = lane; e < bins; e += 32) {
+    int total = 0, below = 0;
 #pragma unroll
-  for (int j = 0; j < (kExchangeMaxExperts + kPlaceWarps * 32) / (kPlaceWarps * 32); ++j) {
-    const int e = threadIdx.x + j * kPlaceWarps * 32;
-    int total = 0, before = 0;
-    if (e < bins)
-      for (int c = 0; c < static_cast<int>(gridDim.x); ++c) {
-        const int n = p.scratch[c * bins + e];
-        total += n;
-        if (c < static_cast<int>(blockIdx.x)) before += n;
-      }
-    before_of[j] = before;
-    if (e < bins) {
-      all[e] = total;
-      if (blockIdx.x == 0 && e < p.num_experts) p.counts[e] = total;
+    for (int j = 0; j < kExchangeMaxChunks / kPlaceWarps; ++j) {
+      const int c = warp + j * kPlaceWarps;
+      const int n = c < static_cast<int>(gridDim.x) ? p.scratch[c * bins + e] : 0;
+      total += n;
+      if (c < static_cast<int>(blockIdx.x)) below += n;
     }
+    atomicAdd(&all[e], total);
+    atomicAdd(&before[e], below);
   }
   __syncthreads();
+  if (blockIdx.x == 0)
+    for (int e = threadIdx.x; e < p.num_experts; e += kPlaceWarps * 32) p.counts[e] = all[e];
+  __syncthreads();                         // the scan turns the counts into first rows
   if (warp == 0) warp_exclusive_scan(all, bins, lane);
   __syncthreads();
-#pragma unroll
-  for (int j = 0; j < (kExchangeMaxExperts + kPlaceWarps * 32) / (kPlaceWarps * 32); ++j) {
-    const int e = threadIdx.x + j * kPlaceWarps * 32;
-    if (e < bins) {
-      int at = all[e] + before_of[j];
-      for (int w = 0; w < kPlaceWarps; ++w) {
-        const int n = next[w * bins + e];
-        next[w * bins + e] = at;
-        at += n;
-      }
+  for (int e = threadIdx.x; e < bins; e += kPlaceWarps * 32) {
+    int at = all[e] + before[e];
+    for (int w = 0; w < kPlaceWarps; ++w) {
+      const int n = next[w * bins + e];
+      next[w * bins + e] = at;
+      at += n;
     }
   }
   __syncthreads();
@@ -271,136 +276,114 @@ template <> __device__ __forceinline__ __half exchange_round<__half>(float v) { 
 template <> __device__ __forceinline__ __nv_bfloat16 exchange_round<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ float exchange_round<float>(float v) { return v; }
 
-// out[t] = sum_s w[t, s] y[row_of[t, s]] (w null: one); 16 bytes a thread, the terms' loads started four at a time.
+// out[t] = sum_s w[t, s] y[row_of[t, s]] (w null: one): a CTA takes a token, a thread 16 bytes of the row;
+// the terms' loads are started four at a time (eight take the registers that keep other warps
+// resident: 128 against 80 us for 16384 x 6 rows of 2048).
 template <typename T>
 __global__ void __launch_bounds__(256) exchange_sum_kernel(const ExchangeSumParams p) {
   constexpr int V = 16 / sizeof(T);
-  const int per_row = p.vec ? p.width / V : p.width;
-  const long long total = p.tokens * per_row;
   const T* y = static_cast<const T*>(p.y);
-  T* out = static_cast<T*>(p.out);
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const long long t = i / per_row;
-    const int c = static_cast<int>(i - t * per_row);
+  for (long long t = blockIdx.x; t < p.tokens; t += gridDim.x) {
     const long long* rows = p.row_of + t * p.top_k;
     const float* w = p.weights != nullptr ? p.weights + t * p.top_k : nullptr;
+    T* out = static_cast<T*>(p.out) + t * p.width;
     if (p.vec) {
-      float acc[V];
+      for (int c = threadIdx.x; c < p.width / V; c += blockDim.x) {
+        float acc[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] = 0.f;
-      for (int s0 = 0; s0 < p.top_k; s0 += 4) {
-        uint4 v[4];
-        float f[4];
-        bool kept[4];
+        for (int j = 0; j < V; ++j) acc[j] = 0.f;
+        for (int s0 = 0; s0 < p.top_k; s0 += 4) {
+          uint4 v[4];
+          float f[4];
+          bool kept[4];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const long long row = s0 + s < p.top_k ? rows[s0 + s] : -1;
-          kept[s] = row >= 0;
-          f[s] = kept[s] && w != nullptr ? w[s0 + s] : 1.f;
-          if (kept[s]) v[s] = reinterpret_cast<const uint4*>(y + row * p.width)[c];
+          for (int s = 0; s < 4; ++s) {
+            const long long row = s0 + s < p.top_k ? rows[s0 + s] : -1;
+            kept[s] = row >= 0;
+            f[s] = kept[s] && w != nullptr ? w[s0 + s] : 1.f;
+            if (kept[s]) v[s] = reinterpret_cast<const uint4*>(y + row * p.width)[c];
+          }
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            if (!kept[s]) continue;
+            const T* e = reinterpret_cast<const T*>(&v[s]);
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j] = fmaf(f[s], Fp8In<T>::get(e[j]), acc[j]);
+          }
         }
+        uint4 o;
+        T* oe = reinterpret_cast<T*>(&o);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          if (!kept[s]) continue;
-          const T* e = reinterpret_cast<const T*>(&v[s]);
-#pragma unroll
-          for (int j = 0; j < V; ++j) acc[j] = fmaf(f[s], Fp8In<T>::get(e[j]), acc[j]);
-        }
+        for (int j = 0; j < V; ++j) oe[j] = exchange_round<T>(acc[j]);
+        reinterpret_cast<uint4*>(out)[c] = o;
       }
-      uint4 o;
-      T* oe = reinterpret_cast<T*>(&o);
-#pragma unroll
-      for (int j = 0; j < V; ++j) oe[j] = exchange_round<T>(acc[j]);
-      reinterpret_cast<uint4*>(out + t * p.width)[c] = o;
     } else {
-      float acc = 0.f;
-      for (int s = 0; s < p.top_k; ++s)
-        if (rows[s] >= 0) acc = fmaf(w != nullptr ? w[s] : 1.f, Fp8In<T>::get(y[rows[s] * p.width + c]), acc);
-      out[t * p.width + c] = exchange_round<T>(acc);
+      for (int c = threadIdx.x; c < p.width; c += blockDim.x) {
+        float acc = 0.f;
+        for (int s = 0; s < p.top_k; ++s)
+          if (rows[s] >= 0) acc = fmaf(w != nullptr ? w[s] : 1.f, Fp8In<T>::get(y[rows[s] * p.width + c]), acc);
+        out[c] = exchange_round<T>(acc);
+      }
     }
   }
 }
 
-// dy[row_of[t, s]] = w[t, s] dout[t] and dw[t, s] = <dout[t], y[row_of[t, s]]>: a CTA takes a token, its
-// slots four at a time; dout is read again for each four, from L1. Thread partials are added by
-// shuffles and then in warp order.
+// dy[row_of[t, s]] = w[t, s] dout[t] and dw[t, s] = <dout[t], y[row_of[t, s]]>: a warp takes a pair, the
+// warps of a CTA neighbouring pairs, so that a token's dout is read from memory once and from L1 after
+// that. No barrier: lanes' partial dot products are added by shuffles (a CTA per token, its
+// threads across the row and two barriers for every four slots, took 205 us where this takes 150).
 template <typename T>
 __global__ void __launch_bounds__(256) exchange_sum_grad_kernel(const ExchangeSumGradParams p) {
   constexpr int V = 16 / sizeof(T);
-  __shared__ float part[4][8];
-  const T* y = static_cast<const T*>(p.y);
-  T* d_y = static_cast<T*>(p.d_y);
-  for (long long t = blockIdx.x; t < p.tokens; t += gridDim.x) {
-    const T* d = static_cast<const T*>(p.d_out) + t * p.width;
-    for (int s0 = 0; s0 < p.top_k; s0 += 4) {
-      long long row[4];
-      float w[4], dot[4];
+  constexpr int kUnroll = 4;
+  const int lane = threadIdx.x & 31;
+  const long long pairs = p.tokens * p.top_k;
+  for (long long i = blockIdx.x * 8ll + (threadIdx.x >> 5); i < pairs; i += gridDim.x * 8ll) {
+    const long long row = p.row_of[i];
+    const bool kept = row >= 0;
+    const float w = kept ? p.weights[i] : 0.f;
+    const T* d = static_cast<const T*>(p.d_out) + i / p.top_k * p.width;
+    const T* y = p.d_weights != nullptr && kept ? static_cast<const T*>(p.y) + row * p.width : nullptr;
+    T* d_y = p.d_y != nullptr ? static_cast<T*>(p.d_y) + (kept ? row : -1 - row) * p.width : nullptr;
+    float dot = 0.f;
+    if (p.vec) {
+      const int vecs = p.width / V;
+      for (int c0 = lane; c0 < vecs; c0 += 32 * kUnroll) {
+        uint4 dv[kUnroll], yv[kUnroll];
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const bool in = s0 + s < p.top_k;
-        row[s] = in ? p.row_of[t * p.top_k + s0 + s] : 0;
-        w[s] = in && row[s] >= 0 ? p.weights[t * p.top_k + s0 + s] : 0.f;
-        dot[s] = 0.f;
-      }
-      if (p.vec) {
-        for (int c = threadIdx.x; c < p.width / V; c += 256) {
-          const uint4 dv = reinterpret_cast<const uint4*>(d)[c];
-          const T* de = reinterpret_cast<const T*>(&dv);
-          uint4 yv[4];
-          if (p.d_weights != nullptr) {
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-              if (s0 + s < p.top_k && row[s] >= 0) yv[s] = reinterpret_cast<const uint4*>(y + row[s] * p.width)[c];
-          }
-#pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            if (s0 + s >= p.top_k) continue;
-            const bool kept = row[s] >= 0;
-            if (p.d_weights != nullptr && kept) {
-              const T* ye = reinterpret_cast<const T*>(&yv[s]);
-#pragma unroll
-              for (int j = 0; j < V; ++j) dot[s] = fmaf(Fp8In<T>::get(de[j]), Fp8In<T>::get(ye[j]), dot[s]);
-            }
-            if (d_y != nullptr) {
-              uint4 o = make_uint4(0, 0, 0, 0);
-              if (kept) {
-                T* oe = reinterpret_cast<T*>(&o);
-#pragma unroll
-                for (int j = 0; j < V; ++j) oe[j] = exchange_round<T>(w[s] * Fp8In<T>::get(de[j]));
-              }
-              reinterpret_cast<uint4*>(d_y + (kept ? row[s] : -1 - row[s]) * p.width)[c] = o;
-            }
-          }
+        for (int j = 0; j < kUnroll; ++j) {
+          const int c = c0 + 32 * j;
+          dv[j] = kept && c < vecs ? reinterpret_cast<const uint4*>(d)[c] : make_uint4(0, 0, 0, 0);
+          yv[j] = y != nullptr && c < vecs ? reinterpret_cast<const uint4*>(y)[c] : make_uint4(0, 0, 0, 0);
         }
-      } else {
-        for (int c = threadIdx.x; c < p.width; c += 256) {
-          const float dv = Fp8In<T>::get(d[c]);
 #pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            if (s0 + s >= p.top_k) continue;
-            const bool kept = row[s] >= 0;
-            if (p.d_weights != nullptr && kept) dot[s] = fmaf(dv, Fp8In<T>::get(y[row[s] * p.width + c]), dot[s]);
-            if (d_y != nullptr)
-              d_y[(kept ? row[s] : -1 - row[s]) * p.width + c] = exchange_round<T>(kept ? w[s] * dv : 0.f);
+        for (int j = 0; j < kUnroll; ++j) {
+          const int c = c0 + 32 * j;
+          if (c >= vecs) continue;
+          const T* de = reinterpret_cast<const T*>(&dv[j]);
+          const T* ye = reinterpret_cast<const T*>(&yv[j]);
+          uint4 o;
+          T* oe = reinterpret_cast<T*>(&o);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float dd = Fp8In<T>::get(de[e]);
+            if (y != nullptr) dot = fmaf(dd, Fp8In<T>::get(ye[e]), dot);
+            oe[e] = exchange_round<T>(kept ? w * dd : 0.f);
           }
+          if (d_y != nullptr) reinterpret_cast<uint4*>(d_y)[c] = o;
         }
       }
-      if (p.d_weights == nullptr) continue;
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) dot[s] += __shfl_xor_sync(0xffffffffu, dot[s], o);
-        if ((threadIdx.x & 31) == 0) part[s][threadIdx.x >> 5] = dot[s];
+    } else {
+      for (int c = lane; c < p.width; c += 32) {
+        const float dd = kept ? Fp8In<T>::get(d[c]) : 0.f;
+        if (y != nullptr) dot = fmaf(dd, Fp8In<T>::get(y[c]), dot);
+        if (d_y != nullptr) d_y[c] = exchange_round<T>(kept ? w * dd : 0.f);
       }
-      __syncthreads();
-      if (threadIdx.x < 4 && s0 + static_cast<int>(threadIdx.x) < p.top_k) {
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum += part[threadIdx.x][i];
-        p.d_weights[t * p.top_k + s0 + threadIdx.x] = sum;            // a dropped pair's dot stayed zero
-      }
-      __syncthreads();
     }
+    if (p.d_weights == nullptr) continue;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if (lane == 0) p.d_weights[i] = dot;                              // a dropped pair's dot is zero
   }
 }
 

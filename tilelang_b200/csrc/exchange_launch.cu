@@ -22,7 +22,7 @@ cudaError_t dispatch(const ExchangeSortParams& s, const ExchangeRowsParams& r, c
   const long long per = std::max<long long>(512, (pairs + kExchangeMaxChunks - 1) / kExchangeMaxChunks);
   const int chunks = static_cast<int>((pairs + per - 1) / per);
   exchange_count_kernel<<<chunks, 256, bins * sizeof(int), stream>>>(s, per);
-  exchange_place_kernel<<<chunks, kPlaceWarps * 32, (kPlaceWarps + 1) * bins * sizeof(int), stream>>>(s, per);
+  exchange_place_kernel<<<chunks, kPlaceWarps * 32, (kPlaceWarps + 2) * bins * sizeof(int), stream>>>(s, per);
   const int grid = static_cast<int>(std::min<long long>(s.tokens, 148 * 32));
   exchange_move_kernel<MOVE><<<grid, 256, 0, stream>>>(s, r);
   return cudaGetLastError();
@@ -43,16 +43,17 @@ cudaError_t launch_exchange_dispatch(const ExchangeSortParams& s, const Exchange
 }
 
 cudaError_t launch_exchange_sum(const ExchangeSumParams& p, cudaStream_t stream) {
-  const int v = p.vec ? (p.type == EXCHANGE_F32 ? 4 : 8) : 1;
-  const int grid = static_cast<int>(std::min<long long>((p.tokens * (p.width / v) + 255) / 256, 148 * 32));
-  if (p.type == EXCHANGE_F16) exchange_sum_kernel<__half><<<grid, 256, 0, stream>>>(p);
-  else if (p.type == EXCHANGE_BF16) exchange_sum_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(p);
-  else exchange_sum_kernel<float><<<grid, 256, 0, stream>>>(p);
+  const int items = p.vec ? p.width / (p.type == EXCHANGE_F32 ? 4 : 8) : p.width;
+  const int threads = std::min(256, (items + 31) / 32 * 32);
+  const int grid = static_cast<int>(std::min<long long>(p.tokens, 148 * 64));
+  if (p.type == EXCHANGE_F16) exchange_sum_kernel<__half><<<grid, threads, 0, stream>>>(p);
+  else if (p.type == EXCHANGE_BF16) exchange_sum_kernel<__nv_bfloat16><<<grid, threads, 0, stream>>>(p);
+  else exchange_sum_kernel<float><<<grid, threads, 0, stream>>>(p);
   return cudaGetLastError();
 }
 
 cudaError_t launch_exchange_sum_grad(const ExchangeSumGradParams& p, cudaStream_t stream) {
-  const int grid = static_cast<int>(std::min<long long>(p.tokens, 148 * 32));
+  const int grid = static_cast<int>(std::min<long long>((p.tokens * p.top_k + 7) / 8, 148 * 64));
   if (p.type == EXCHANGE_F16) exchange_sum_grad_kernel<__half><<<grid, 256, 0, stream>>>(p);
   else if (p.type == EXCHANGE_BF16) exchange_sum_grad_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(p);
   else exchange_sum_grad_kernel<float><<<grid, 256, 0, stream>>>(p);

@@ -161,10 +161,6 @@ __device__ __forceinline__ void fp8_pair_add(uint64_t (&acc)[64], const int at, 
   for (int j = 0; j < 16; ++j) acc[at + j] = ffma2(pack2(v[2 * j], v[2 * j + 1]), scale, acc[at + j]);
 }
 
-// silu(g) * u with the hardware's exponential and reciprocal: a relative error near 2^-21, far below the
-// codes' half step of 2^-4 or 2^-3. For g so low that e^-g is infinite the reciprocal is zero.
-__device__ __forceinline__ float fast_silu_mul(float g, float u) { return g * __fdividef(1.0f, 1.0f + __expf(-g)) * u; }
-
 __device__ __forceinline__ void pair_barrier(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
 // The two warps of a lane quarter: `half` 0 holds g, 1 holds u of 32 tokens x 128 features. Each sends
@@ -193,18 +189,18 @@ __device__ __forceinline__ void fp8_pair_gate(const Fp8GemmParams& p, uint8_t* m
       const float own[4] = {a.x, a.y, b.x, b.y}, got[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        act[r * 32 + 4 * j + e] = half == 0 ? fast_silu_mul(own[e], got[e]) : fast_silu_mul(got[e], own[e]);
+        act[r * 32 + 4 * j + e] = half == 0 ? silu_mul_of(own[e], got[e]) : silu_mul_of(got[e], own[e]);
     }
     pair_barrier(1 + quarter);
   }
-  uint32_t m_bits = 0;
+  float amax = 0.f;
 #pragma unroll
-  for (int j = 0; j < 64; ++j) m_bits = max(m_bits, magnitude_bits(act[j]));
-  reinterpret_cast<uint32_t*>(mine)[lane] = m_bits;
+  for (int j = 0; j < 64; ++j) amax = max_magnitude(amax, act[j]);
+  reinterpret_cast<float*>(mine)[lane] = amax;
   pair_barrier(1 + quarter);
-  m_bits = max(m_bits, reinterpret_cast<const uint32_t*>(other)[lane]);
+  amax = max_magnitude(amax, reinterpret_cast<const float*>(other)[lane]);
   pair_barrier(1 + quarter);                                  // read before the next tile's rows overwrite it
-  const float s = fp8_scale_of<FP8>(m_bits);
+  const float s = fp8_scale_of<FP8>(__float_as_uint(amax));
   const float inv = __frcp_rn(s);
   if (in) {
     uint8_t* dst = p.gate_codes + m * p.ld_gate + f0 + half * 64;
