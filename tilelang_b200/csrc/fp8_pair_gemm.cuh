@@ -86,11 +86,11 @@ __device__ __forceinline__ void fp8_pair_prefixes(const Fp8GemmParams& p, Fp8Pai
   if (lane == 0) ctl->row_prefix[0] = ctl->tile_prefix[0] = 0;
 }
 
-// Where tile t lies: strips of kPairStrip token tiles, within a strip token tiles fastest.
-__device__ __forceinline__ Fp8Tile fp8_pair_tile(const Fp8GemmParams& p, const Fp8PairCtl* ctl, int token_tiles, long long t) {
-  const long long strip_tiles = static_cast<long long>(kPairStrip) * p.p_tiles;
-  const int strip = static_cast<int>(t / strip_tiles);
-  const int in_strip = static_cast<int>(t - strip * strip_tiles);
+// Where tile t lies: strips of kPairStrip token tiles, within a strip token tiles fastest. (The output has
+// 65536 elements a tile, so the tiles of any output that fits the GPU can be counted in 32 bits.)
+__device__ __forceinline__ Fp8Tile fp8_pair_tile(const Fp8GemmParams& p, const Fp8PairCtl* ctl, int token_tiles, int t) {
+  const int strip = t / (kPairStrip * p.p_tiles);
+  const int in_strip = t - strip * (kPairStrip * p.p_tiles);
   const int high = min(kPairStrip, token_tiles - strip * kPairStrip);
   const int tt = strip * kPairStrip + in_strip % high;
   const int p0 = in_strip / high * p.tile_cols;
@@ -103,55 +103,72 @@ __device__ __forceinline__ Fp8Tile fp8_pair_tile(const Fp8GemmParams& p, const F
   return Fp8Tile{lo, ctl->row_prefix[lo] + (tt - ctl->tile_prefix[lo]) * 256, ctl->row_prefix[lo + 1], p0};
 }
 
+__device__ __forceinline__ void st_shared4(uint32_t addr, const uint32_t (&v)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
 // 32 rows x 128 columns of fp32 sums (thread = row) to C, 128 bytes of each row at a time through the
 // warp's 4 KB of shared memory (16-byte chunks rotated by the row: no bank conflicts either way).
 template <int OUT_TYPE>
-__device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, uint8_t* stage, const uint64_t (&acc)[64],
+__device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, uint32_t stage, const uint64_t (&acc)[64],
                                                long long m_first, int rows, int col0, int lane) {
   constexpr int kSize = OUT_TYPE == OUT_F32 ? 4 : 2;
   constexpr int kCols = 128 / kSize;                          // columns of a pass
+  const uint32_t out_at = stage + lane * 128, out_rot = (lane & 7) << 4;
+  const int chunk = lane & 7, row0 = lane >> 3;
+  const long long pitch = p.ldc * kSize;
+  uint8_t* dst = static_cast<uint8_t*>(p.c) + (m_first + row0) * pitch + (col0 + chunk * (16 / kSize)) * kSize;
 #pragma unroll
   for (int pass = 0; pass < 128 / kCols; ++pass) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {                             // 16-byte chunks of this thread's row
-      uint4 v;
-      if (OUT_TYPE == OUT_F32) {
-        const float2 a = unpack2(acc[pass * 16 + 2 * j]), b = unpack2(acc[pass * 16 + 2 * j + 1]);
-        v = make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
-      } else {
-        uint32_t h[4];
+      uint32_t h[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 4; ++i) {
+        if (OUT_TYPE == OUT_F32) {
+          const float2 f = unpack2(acc[pass * 16 + 2 * j + (i >> 1)]);
+          h[i] = __float_as_uint(i & 1 ? f.y : f.x);
+        } else {
           const float2 f = unpack2(acc[pass * 32 + 4 * j + i]);
           h[i] = OUT_TYPE == OUT_BF16 ? bf162_as_u32(__floats2bfloat162_rn(f.x, f.y)) : h2_as_u32(__floats2half2_rn(f.x, f.y));
         }
-        v = make_uint4(h[0], h[1], h[2], h[3]);
       }
-      *reinterpret_cast<uint4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = v;
+      st_shared4(out_at + ((j << 4) ^ out_rot), h);
     }
     __syncwarp();
-    const int chunk = lane & 7;
-    const int col = col0 + pass * kCols + chunk * (16 / kSize);
+    uint4 v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int row = i * 4 + (lane >> 3);
-      const uint4 v = *reinterpret_cast<const uint4*>(stage + row * 128 + ((chunk ^ (row & 7)) << 4));
-      if (row < rows && col < p.P) {
-        uint8_t* dst = static_cast<uint8_t*>(p.c) + (static_cast<size_t>(m_first + row) * p.ldc + col) * kSize;
-        if (p.c_vec16) {
-          *reinterpret_cast<uint4*>(dst) = v;
-        } else {
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      const int row = i * 4 + row0;
+      v[i] = ld_shared4(stage + row * 128 + ((chunk ^ (row & 7)) << 4));
+    }
+    __syncwarp();
+    const int col = col0 + pass * kCols + chunk * (16 / kSize);
+    if (col < p.P) {
+      if (p.c_vec16) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i * 4 + row0 < rows) *reinterpret_cast<uint4*>(dst + i * 4 * pitch) = v[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (i * 4 + row0 >= rows) continue;
+          const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
           for (int e = 0; e < 16 / kSize; ++e) {
             if (col + e >= p.P) break;
-            if (kSize == 4) reinterpret_cast<uint32_t*>(dst)[e] = w[e];
-            else reinterpret_cast<uint16_t*>(dst)[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+            if (kSize == 4) reinterpret_cast<uint32_t*>(dst + i * 4 * pitch)[e] = w[e];
+            else reinterpret_cast<uint16_t*>(dst + i * 4 * pitch)[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
           }
         }
       }
     }
-    __syncwarp();
+    dst += 128;
   }
 }
 
@@ -167,7 +184,7 @@ __device__ __forceinline__ void pair_barrier(int id) { asm volatile("bar.sync %0
 // the half that the other one works on (32 columns at a time, 16-byte chunks rotated by the row), then
 // quantises its 64 features. `mine`, `other`: their 4 KB of shared memory.
 template <int FP8>
-__device__ __forceinline__ void fp8_pair_gate(const Fp8GemmParams& p, uint8_t* mine, const uint8_t* other, const uint64_t (&acc)[64],
+__device__ __forceinline__ void fp8_pair_gate(const Fp8GemmParams& p, uint32_t mine, uint32_t other, const uint64_t (&acc)[64],
                                               int half, int quarter, long long m, bool in, int f0, int lane) {
   float act[64];
 #pragma unroll
@@ -178,27 +195,33 @@ __device__ __forceinline__ void fp8_pair_gate(const Fp8GemmParams& p, uint8_t* m
       const uint64_t lo = half == 0 ? acc[32 + r * 16 + 2 * j] : acc[r * 16 + 2 * j];
       const uint64_t hi = half == 0 ? acc[32 + r * 16 + 2 * j + 1] : acc[r * 16 + 2 * j + 1];
       const float2 a = unpack2(lo), b = unpack2(hi);
-      *reinterpret_cast<float4*>(mine + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(a.x, a.y, b.x, b.y);
+      const uint32_t w[4] = {__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y)};
+      st_shared4(mine + lane * 128 + ((j ^ (lane & 7)) << 4), w);
     }
     pair_barrier(1 + quarter);
+    uint4 in4[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) in4[j] = ld_shared4(other + lane * 128 + ((j ^ (lane & 7)) << 4));
+    pair_barrier(1 + quarter);                                // the partner may write again
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float4 o = *reinterpret_cast<const float4*>(other + lane * 128 + ((j ^ (lane & 7)) << 4));
+      const uint4 o = in4[j];
       const float2 a = unpack2(half == 0 ? acc[r * 16 + 2 * j] : acc[32 + r * 16 + 2 * j]);
       const float2 b = unpack2(half == 0 ? acc[r * 16 + 2 * j + 1] : acc[32 + r * 16 + 2 * j + 1]);
-      const float own[4] = {a.x, a.y, b.x, b.y}, got[4] = {o.x, o.y, o.z, o.w};
+      const float own[4] = {a.x, a.y, b.x, b.y}, got[4] = {__uint_as_float(o.x), __uint_as_float(o.y), __uint_as_float(o.z), __uint_as_float(o.w)};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         act[r * 32 + 4 * j + e] = half == 0 ? silu_mul_of(own[e], got[e]) : silu_mul_of(got[e], own[e]);
     }
-    pair_barrier(1 + quarter);
   }
   float amax = 0.f;
 #pragma unroll
   for (int j = 0; j < 64; ++j) amax = max_magnitude(amax, act[j]);
-  reinterpret_cast<float*>(mine)[lane] = amax;
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + lane * 4), "f"(amax) : "memory");
   pair_barrier(1 + quarter);
-  amax = max_magnitude(amax, reinterpret_cast<const float*>(other)[lane]);
+  float partner;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(partner) : "r"(other + lane * 4) : "memory");
+  amax = max_magnitude(amax, partner);
   pair_barrier(1 + quarter);                                  // read before the next tile's rows overwrite it
   const float s = fp8_scale_of<FP8>(__float_as_uint(amax));
   const float inv = __frcp_rn(s);
@@ -250,7 +273,7 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   tc_fence_after_sync();
   const uint32_t tmem_base = ctl->tmem_base;
   const int token_tiles = p.counts != nullptr ? ctl->tile_prefix[p.num_groups] : (p.M + 255) / 256;
-  const long long tiles = static_cast<long long>(token_tiles) * p.p_tiles;
+  const int tiles = token_tiles * p.p_tiles;
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   if (warp < 4) {
@@ -259,7 +282,7 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       // ---------------- producer: this CTA's halves, completing on the first CTA's barriers ----------------
       uint32_t s = 0, phase = 0;
       bool ok = true;
-      for (long long t = pair; ok && t < tiles; t += pairs) {
+      for (int t = pair; ok && t < tiles; t += pairs) {
         const Fp8Tile tile = fp8_pair_tile(p, ctl, token_tiles, t);
         const int m0 = tile.m0 + rank * 128, p0 = tile.p0 + rank * (GATED ? p.P / 2 : 128);
         for (int kb = 0; kb < p.q_blocks; ++kb) {
@@ -280,7 +303,7 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       const uint64_t w_step = p.trans_w ? 32 * 128 / 16 : 2;
       uint32_t s = 0, phase = 0, i = 0;
       bool ok = true;
-      for (long long t = pair; t < tiles; t += pairs) {
+      for (int t = pair; t < tiles; t += pairs) {
         for (int kb = 0; kb < p.q_blocks; ++kb, ++i) {
           const uint32_t buf = i & 1u, acc = tmem_base + buf * 256;
           const uint32_t stage = smem_u32(smem + s * kPairStageBytes);
@@ -305,25 +328,32 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     // ---------------- sums: thread = one token of this CTA, 128 of the tile's columns ----------------
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-    uint8_t* stage = stage_out + (warp - 4) * kPairStageOut;
+    const uint32_t stage = smem_u32(stage_out + (warp - 4) * kPairStageOut);
+    const uint32_t other = smem_u32(stage_out + ((warp - 4) ^ 4) * kPairStageOut);
     const uint32_t empty_bar = cluster_map(smem_u32(&ctl->acc_empty[0]), 0);
     const uint32_t acc_addr = tmem_base + lane_addr + half * 128;
     uint32_t i = 0;
     bool ok = true;
-    for (long long t = pair; t < tiles; t += pairs) {
-      const Fp8Tile tile = fp8_pair_tile(p, ctl, token_tiles, t);
-      const int m_first = tile.m0 + rank * 128 + quarter * 32;
+    // What a tile needs from memory: its scales, two blocks ahead (their latency is longer than a block's
+    // multiplication). The next tile's first two are fetched before this one's rows are written.
+    Fp8Tile tile;
+    const float *as = nullptr, *ws = nullptr;
+    float a0 = 0.f, w0 = 0.f, a1 = 0.f, w1 = 0.f;
+    const auto begin = [&](int t) {
+      tile = fp8_pair_tile(p, ctl, token_tiles, t);
       // a tile may end before its second half; gated, the second half is the up half of the weight
       const int p_block = GATED ? (tile.p0 + half * (p.P / 2)) / 128 : min(tile.p0 / 128 + half, (p.P - 1) / 128);
-      const float* as = p.a_scale + static_cast<long long>(min(m_first + lane, p.M - 1)) * p.ld_a_scale;
-      const float* ws = p.w_scale + tile.group * p.ws_group + p_block * p.ws_p;
+      as = p.a_scale + static_cast<long long>(min(tile.m0 + rank * 128 + quarter * 32 + lane, p.M - 1)) * p.ld_a_scale;
+      ws = p.w_scale + tile.group * p.ws_group + p_block * p.ws_p;
+      a0 = as[0]; w0 = ws[0];
+      if (p.q_blocks > 1) { a1 = as[1]; w1 = ws[p.ws_q]; }
+      as += 2; ws += 2 * p.ws_q;
+    };
+    if (pair < tiles) begin(pair);
+    for (int t = pair; t < tiles; t += pairs) {
       uint64_t acc[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) acc[j] = 0;
-      // the scales two blocks ahead: their latency is longer than a block's multiplication
-      float a0 = as[0], w0 = ws[0], a1 = 0.f, w1 = 0.f;
-      if (p.q_blocks > 1) { a1 = as[1]; w1 = ws[p.ws_q]; }
-      as += 2; ws += 2 * p.ws_q;
       // Two pieces of 32 columns are in registers or on their way at any time; the order hands the accumulator
       // back after half of the additions and fetches the next block's first half under the other half.
       uint32_t v[2][32];
@@ -365,19 +395,21 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         if (more) tmem_ld_32x32b_x32(next + 32, v[1]);
         a0 = a1; w0 = w1; a1 = a2; w1 = w2;
       }
-      const int rows = min(32, tile.m_end - m_first);
+      const Fp8Tile done = tile;
+      if (t + pairs < tiles) begin(t + pairs);
+      const int m_first = done.m0 + rank * 128 + quarter * 32;
+      const int rows = min(32, done.m_end - m_first);
       if (GATED) {
         // both warps of a quarter meet in here, whatever happened to either
-        const uint8_t* other = stage_out + ((warp - 4) ^ 4) * kPairStageOut;
         const bool in = ok && lane < rows;
         if (p.gate_fp8 == FP8_E4M3)
-          fp8_pair_gate<FP8_E4M3>(p, stage, other, acc, half, quarter, m_first + lane, in, tile.p0, lane);
+          fp8_pair_gate<FP8_E4M3>(p, stage, other, acc, half, quarter, m_first + lane, in, done.p0, lane);
         else
-          fp8_pair_gate<FP8_E5M2>(p, stage, other, acc, half, quarter, m_first + lane, in, tile.p0, lane);
+          fp8_pair_gate<FP8_E5M2>(p, stage, other, acc, half, quarter, m_first + lane, in, done.p0, lane);
         if (ok && p.c != nullptr)
-          fp8_pair_store<OUT_BF16>(p, stage, acc, m_first, rows, tile.p0 + half * (p.P / 2), lane);
+          fp8_pair_store<OUT_BF16>(p, stage, acc, m_first, rows, done.p0 + half * (p.P / 2), lane);
       } else if (ok) {
-        const int col0 = tile.p0 + half * 128;
+        const int col0 = done.p0 + half * 128;
         if (p.out_type == OUT_BF16) fp8_pair_store<OUT_BF16>(p, stage, acc, m_first, rows, col0, lane);
         else if (p.out_type == OUT_F16) fp8_pair_store<OUT_F16>(p, stage, acc, m_first, rows, col0, lane);
         else fp8_pair_store<OUT_F32>(p, stage, acc, m_first, rows, col0, lane);
