@@ -291,7 +291,7 @@ typedef struct b200dq_fp8_gemm_args {
   int32_t a_type, w_type;   /* enum b200dq_fp8_type, any pairing                              */
   int32_t out_type;         /* f16, bf16 or f32                                               */
   int32_t trans_w;
-  int32_t token_tile;       /* 0: chosen; 16, 32, 64: tokens are the tile's columns, 128: its lanes, 256: a CTA pair's */
+  int32_t token_tile;       /* 0: chosen; 16, 32: tokens are the tile's columns, 128: its lanes, 256: a CTA pair's */
   int32_t split;            /* 0: chosen; else CTAs (1 to 8) that share a tile's contraction  */
   /* Gated (NULL for none): N = 2F rows of W, gate above up, F a multiple of 128. Instead of h = A * W^T
    * the codes and scales of silu(h[:, :F]) * h[:, F:] are written, from the fp32 sums; c may be NULL,

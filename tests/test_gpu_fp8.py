@@ -173,7 +173,7 @@ def test_product_of_either_type(a_type, w_type, M, trans):
     check_product(c, a, a_scale, w.codes, w.scales, trans)
 
 
-@pytest.mark.parametrize("token_tile", [16, 32, 64, 128])
+@pytest.mark.parametrize("token_tile", [16, 32, 128])
 @pytest.mark.parametrize("split", [1, 2, 3, 5, 8])
 @pytest.mark.parametrize("trans", [False, True])
 def test_every_tile_and_split(token_tile, split, trans):
@@ -198,7 +198,7 @@ def test_tiles_of_cta_pairs(M, N, K, trans, out_dtype):
     assert torch.equal(c, ops.gemm_fp8(a, a_scale, w, trans_w=trans, out_dtype=out_dtype, token_tile=256))
 
 
-@pytest.mark.parametrize("token_tile", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("token_tile", [16, 32, 128, 256])
 @pytest.mark.parametrize("trans", [False, True])
 def test_one_hot_rows_read_the_weight_back(token_tile, trans):
     """A row of one 1 and scales that are powers of two give the weight's values, bit for bit."""
@@ -240,7 +240,7 @@ def test_infinities_stay_in_their_rows():
     x[3, 5], x[7, 300] = float("inf"), float("nan")
     a, a_scale = ops.quant_fp8(x)
     w = ops.quant_fp8_weight(randn(256, 512, seed=4))
-    for tile in (16, 32, 64, 128, 256):
+    for tile in (16, 32, 128, 256):
         c = ops.gemm_fp8(a, a_scale, w, token_tile=tile)
         bad = torch.zeros(40, dtype=torch.bool, device=DEV)
         bad[[3, 7]] = True
@@ -266,7 +266,7 @@ COUNTS = [[1], [0, 3, 0], [300, 0, 17, 256, 1], [40, 90, 33], [1] * 40, [0] * 35
 
 @pytest.mark.parametrize("counts", COUNTS)
 @pytest.mark.parametrize("trans", [False, True])
-@pytest.mark.parametrize("token_tile", [0, 16, 64, 128, 256])
+@pytest.mark.parametrize("token_tile", [0, 16, 32, 128, 256])
 def test_grouped_product(counts, trans, token_tile):
     """Empty experts, single rows, exact tiles; rows behind the last expert stay as they were."""
     N, K = 144, 272

@@ -492,34 +492,48 @@ int run_gemm(const char* who, const b200dq_gemm_args* a, void* scratch, size_t s
 // ---- block-scaled fp8 products ---------------------------------------------------------------
 
 struct Fp8Plan {
-  int token_tile;        // 16, 32, 64: tokens in columns; 128: tokens on lanes; 256: CTA pairs
-  int split;
-  long long tiles;       // clusters to launch (an upper bound when the counts are on the device)
+  int token_tile;        // 16, 32: tokens in columns; 128: tokens on lanes; 256: CTA pairs
+  int p_tiles;           // tiles along the output's columns
+  long long tiles;       // an upper bound when the counts are on the device
 };
 
-// Token tile and split of a product with `rows` rows (in `groups` groups, or 0), `p_tiles` tiles of 128
-// output columns and `q_blocks` blocks of contraction.
-//  - Tile: tokens in columns as long as a tile holds them all (a group's mean share, when grouped): the weights
-//    are then read once and the tensor cores' 128 lanes are full of them. From 65 tokens on they fill the
-//    lanes themselves, and a reading thread's scale is one number instead of a vector.
-//  - Split: as many CTAs as the GPU holds at once (two per SM below 128 tokens), at most 8 per tile (the
-//    portable cluster size), each with at least two blocks.
-Fp8Plan plan_fp8(int rows, int groups, int p_tiles, int q_blocks, int sms, int token_tile, int split) {
+// Token tile of a product with `rows` rows (in `groups` groups, or 0) and `p_blocks` blocks of 128 output columns:
+//  - tokens in columns of 16 or 32 as long as one tile holds them all (a group's mean share, when grouped):
+//    the weights are then read once, and lanes are full of them;
+//  - from 33 tokens on they own the lanes, half empty or not (measured in fp8_gemm.cuh);
+//  - from 129 tokens on CTA pairs with 256 x 256 tiles, unless there are so few of them that half the SMs
+//    would have none (256 tokens, 4096 x 4096: 14 us with 128-token tiles, 19 with pairs; at 14336
+//    rows of weight 36 and 21).
+Fp8Plan plan_fp8(int rows, int groups, int p_blocks, int sms, int token_tile) {
   Fp8Plan plan;
   const long long share = groups > 0 ? (rows + groups - 1) / groups : rows;
-  plan.token_tile = token_tile > 0 ? token_tile : share <= 16 ? 16 : share <= 32 ? 32 : share <= 64 ? 64 : 128;
+  const int pair_tiles = (p_blocks + 1) / 2;
+  plan.token_tile = token_tile > 0 ? token_tile : share <= 16 ? 16 : share <= 32 ? 32 : 128;
   if (token_tile == 0 && share > 128 && groups <= kFp8PairMaxGroups &&
-      static_cast<long long>((rows + 255) / 256) * ((p_tiles + 1) / 2) * 2 >= sms / 2)
+      ((rows + 255ll) / 256) * pair_tiles * 4 >= sms)
     plan.token_tile = 256;
-  if (plan.token_tile == 256) p_tiles = (p_tiles + 1) / 2;
-  long long token_tiles = (rows + plan.token_tile - 1) / plan.token_tile;
-  if (groups > 0) token_tiles = rows / plan.token_tile + std::min<long long>(groups, rows);
-  plan.tiles = token_tiles * p_tiles;
-  const long long slots = static_cast<long long>(sms) * (plan.token_tile >= 128 ? 1 : 2);
-  long long s = split > 0 ? split : slots / plan.tiles;
-  s = std::min<long long>(s, split > 0 ? q_blocks : q_blocks / 2);
-  plan.split = static_cast<int>(std::max<long long>(1, std::min<long long>(s, 8)));
+  plan.p_tiles = plan.token_tile == 256 ? pair_tiles : p_blocks;
+  const long long token_tiles = groups > 0 ? rows / plan.token_tile + std::min(groups, rows)
+                                           : (rows + plan.token_tile - 1ll) / plan.token_tile;
+  plan.tiles = token_tiles * plan.p_tiles;
   return plan;
+}
+
+// CTAs that share a tile's contraction: the most (at most 8, the portable cluster size, and two blocks each at
+// least) with which all tiles still run at once; a second wave costs more than the split gains (333 tokens,
+// 2048 x 1408: 9 us with clusters of 2, 14 with clusters of 3, of which some wait).
+int split_fp8(const Fp8Plan& plan, int q_blocks, int* split) {
+  *split = 1;
+  for (int s = std::min(8, q_blocks / 2); s > 1; --s) {
+    int clusters = 0;
+    if (plan.tiles * s > 148 * 2 * 4) continue;            // more CTAs than any SM count in sight holds
+    CUDA_OK(fp8_resident_clusters(plan.token_tile, s, &clusters));
+    if (plan.tiles <= clusters) {
+      *split = s;
+      break;
+    }
+  }
+  return 0;
 }
 
 int encode_fp8_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
@@ -554,9 +568,8 @@ int check_fp8_gemm(const b200dq_fp8_gemm_args* a) {
   if ((reinterpret_cast<uintptr_t>(a->a_scale) & 3) != 0 || (reinterpret_cast<uintptr_t>(a->w_scale) & 3) != 0 ||
       (reinterpret_cast<uintptr_t>(a->c) & (out_elem_size(a->out_type) - 1)) != 0)
     return fail("gemm_fp8: scales and output must be aligned to their elements");
-  if (a->token_tile != 0 && a->token_tile != 16 && a->token_tile != 32 && a->token_tile != 64 && a->token_tile != 128 &&
-      a->token_tile != 256)
-    return fail("gemm_fp8: token_tile must be 0, 16, 32, 64, 128 or 256 (got %d)", a->token_tile);
+  if (a->token_tile != 0 && a->token_tile != 16 && a->token_tile != 32 && a->token_tile != 128 && a->token_tile != 256)
+    return fail("gemm_fp8: token_tile must be 0, 16, 32, 128 or 256 (got %d)", a->token_tile);
   if (a->token_tile == 256 && a->num_groups > kFp8PairMaxGroups)
     return fail("gemm_fp8: the 256-token tile takes at most %d groups", kFp8PairMaxGroups);
   if (a->token_tile == 256 && a->split > 1) return fail("gemm_fp8: the 256-token tile does not split the contraction");
@@ -587,7 +600,6 @@ int run_gemm_fp8(const b200dq_fp8_gemm_args* a, const DeviceState* ds, cudaStrea
   p.ldc = outer;
   p.M = a->M; p.P = outer;
   p.q_blocks = (inner + 127) / 128;
-  p.p_tiles = (outer + 127) / 128;
   p.out_type = a->out_type;
   p.a_fmt = a->a_type; p.w_fmt = a->w_type;
   p.trans_w = a->trans_w ? 1 : 0;
@@ -598,8 +610,10 @@ int run_gemm_fp8(const b200dq_fp8_gemm_args* a, const DeviceState* ds, cudaStrea
   p.num_groups = a->num_groups;
   p.status = ds->status;
   const bool gated = a->gate_codes != nullptr;
-  const Fp8Plan plan = plan_fp8(a->M, a->num_groups, p.p_tiles, p.q_blocks, ds->sm_count, gated ? 256 : a->token_tile, a->split);
-  p.split = plan.split;
+  const Fp8Plan plan = plan_fp8(a->M, a->num_groups, (outer + 127) / 128, ds->sm_count, gated ? 256 : a->token_tile);
+  p.p_tiles = plan.p_tiles;
+  p.split = std::min(a->split, p.q_blocks);
+  if (p.split == 0 && plan.token_tile < 256 && split_fp8(plan, p.q_blocks, &p.split) != 0) return -1;
   CUtensorMap tmap_a, tmap_w;
   const cuuint64_t a_dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(a->M)};
   const cuuint64_t a_strides[1] = {static_cast<cuuint64_t>(a->lda)};
@@ -610,7 +624,6 @@ int run_gemm_fp8(const b200dq_fp8_gemm_args* a, const DeviceState* ds, cudaStrea
                                    static_cast<cuuint64_t>(groups > 1 ? a->w_group_stride : a->ldw * a->N)};
   if (encode_fp8_map(&tmap_w, a->w, 3, w_dims, w_strides, kFp8BoxRows) != 0) return -1;
   if (plan.token_tile == 256) {
-    p.p_tiles = (p.p_tiles + 1) / 2;
     p.tile_cols = gated ? 128 : 256;
     p.gate_codes = static_cast<uint8_t*>(a->gate_codes);
     p.gate_scales = a->gate_scales;
@@ -1006,7 +1019,7 @@ int b200dq_gemm_fp8(const b200dq_fp8_gemm_args* a, void* cuda_stream) {
 
 int b200dq_fp8_gated_fuses(int32_t M, int32_t N, int32_t K, int32_t num_groups) {
   if (M <= 0 || N <= 0 || K <= 0 || N % 256 != 0 || num_groups < 0) return 0;
-  return plan_fp8(M, num_groups, N / 128, (K + 127) / 128, sm_count_or_bound(), 0, 0).token_tile == 256 ? 1 : 0;
+  return plan_fp8(M, num_groups, N / 128, sm_count_or_bound(), 0).token_tile == 256 ? 1 : 0;
 }
 
 size_t b200dq_exchange_scratch_bytes(int64_t tokens, int32_t top_k, int32_t num_experts) {

@@ -92,11 +92,13 @@ __device__ __forceinline__ void fp8_store4(const Fp8GemmParams& p, long long m, 
 // ---- one tile per cluster, its contraction split over the cluster's CTAs ---------------------------
 //
 // For few tokens and for problems of fewer tiles than the GPU has SMs. TN tokens x 128 weight rows:
-//   TOK_LANE = false: weights own the 128 lanes (the instruction's M), tokens its N = TN columns, so a
-//     token costs a column and not a lane; token scales reach the reading warps through a ring of TN
+//   TOK_LANE = false, TN = 16 or 32: weights own the 128 lanes (the instruction's M), tokens its N = TN
+//     columns, so a token costs a column and not a lane; token scales reach the reading warps through a ring of TN
 //     floats per block in shared memory, filled by 4-byte asynchronous copies.
-//   TOK_LANE = true: tokens own the lanes, 128 weight rows the columns; a reading thread then has one
-//     token and one scale per block (no vector of scales, half the fp32 work).
+//   TOK_LANE = true, TN = 128: tokens own the lanes, 128 weight rows the columns; a reading thread then
+//     has one token and one scale per block (no vector of scales, half the fp32 work). Faster from 33
+//     tokens on, half empty as it is then (48 tokens, 14336 x 4096: 18 us against 22 in columns of 32 and 31
+//     in columns of 64, which need the vector of scales and more registers than two CTAs an SM leave).
 // A cluster of up to 8 CTAs cuts the contraction, leaves its partial sums in shared memory, and every
 // CTA adds up a share of the tile from all of them in rank order: no scratch, one launch, and the
 // same bits every time.
@@ -104,17 +106,17 @@ __device__ __forceinline__ void fp8_store4(const Fp8GemmParams& p, long long m, 
 // warp 0: TMA producer; warp 1: MMA issuer; warp 2: token scales; warp 3: tensor memory; then 4 or 8
 // reading warps. Waits are bounded.
 template <int TN> struct Fp8TileConfig {
-  static constexpr int kReadWarps = TN >= 64 ? 8 : 4;
+  static constexpr int kReadWarps = TN == 128 ? 8 : 4;
   static constexpr int kThreads = 128 + 32 * kReadWarps;
   static constexpr int kCols = TN / (kReadWarps / 4);              // columns a reading thread adds up
-  static constexpr int kAcc = TN >= 128 ? 2 : 4;                   // accumulators
-  static constexpr int kTmemCols = TN * kAcc;                      // 64, 128, 256, 256: two CTAs fit an SM
+  static constexpr int kAcc = 4;                                   // accumulators: the way round is longer than a block
+  static constexpr int kTmemCols = TN * kAcc;                      // 64, 128, 512
   static constexpr int kTokenBytes = TN * 128;
   static constexpr int kStageBytes = 128 * 128 + kTokenBytes;
-  // Stages: two CTAs per SM below 128 tokens (bytes in flight, and one's start under the other's end), one at
-  // 128, whose reading threads need the registers.
-  static constexpr int kStages = TN == 16 ? 6 : TN == 32 ? 5 : TN == 64 ? 4 : 6;
-  static constexpr int kCtasPerSm = TN >= 128 ? 1 : 2;
+  // Up to 32 tokens two CTAs share an SM (bytes in flight, and one's start under the other's end); at 128
+  // the reading threads need the registers and the four accumulators all of tensor memory.
+  static constexpr int kStages = TN == 32 ? 5 : 6;
+  static constexpr int kCtasPerSm = TN == 128 ? 1 : 2;
   static constexpr int kScaleSlots = 8;
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kScaleSlots * TN * 4 + 512;
 };
@@ -236,7 +238,7 @@ fp8_tile_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     const int col0 = ((warp - 4) >> 2) * C::kCols;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const int row = quarter * 32 + lane;                                // this thread's lane of the accumulator
-    constexpr int kChunk = C::kCols < 16 ? C::kCols : 16;
+    constexpr int kChunk = C::kCols < 32 ? C::kCols : 32;
     uint64_t acc[C::kCols / 2];
 #pragma unroll
     for (int i = 0; i < C::kCols / 2; ++i) acc[i] = 0;
@@ -254,37 +256,42 @@ fp8_tile_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       if (kb + 2 < kb1) { w2 = ws[(kb + 2) * p.ws_q]; if (TOK_LANE) a2 = as[kb + 2]; }
       const float lane_scale = TOK_LANE ? a0 * w0 : w0;
       const uint64_t ls = pack2f(lane_scale, lane_scale);
-      if (!TOK_LANE) ok &= mbar_wait_warp(&ctl->sc_full[s], phase, abort_flag, st, 5, lane);
-      ok &= mbar_wait_warp(&ctl->acc_full[buf], (i / C::kAcc) & 1u, abort_flag, st, 6, lane);
+      if (!TOK_LANE) ok &= mbar_wait(&ctl->sc_full[s], phase, abort_flag, st, 5);
+      ok &= mbar_wait(&ctl->acc_full[buf], (i / C::kAcc) & 1u, abort_flag, st, 6);
+      __syncwarp();
       tc_fence_after_sync();
+      // all of this thread's columns at once: one latency of tensor memory a block, not one per piece
+      uint32_t v[C::kCols / kChunk][kChunk];
 #pragma unroll
-      for (int c = 0; c < C::kCols; c += kChunk) {
-        uint32_t v[16];
-        tmem_ld_32x32b_x16(tmem_base + lane_addr + buf * TN + col0 + c, v);
-        uint64_t sc[8];
-        if (!TOK_LANE) {
-          const float4* f = reinterpret_cast<const float4*>(scale_ring + s * TN + col0 + c);
+      for (int c = 0; c < C::kCols / kChunk; ++c) tmem_ld_cols(tmem_base + lane_addr + buf * TN + col0 + c * kChunk, v[c]);
+      uint64_t sc[TOK_LANE ? 1 : C::kCols / 2];
+      if (TOK_LANE) {
+        sc[0] = ls;
+      } else {
+        const float4* f = reinterpret_cast<const float4*>(scale_ring + s * TN + col0);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4 q = f[j];
-            sc[2 * j] = fmul2(pack2f(q.x, q.y), ls);
-            sc[2 * j + 1] = fmul2(pack2f(q.z, q.w), ls);
-          }
+        for (int j = 0; j < C::kCols / 4; ++j) {
+          const float4 q = f[j];
+          sc[(2 * j) % (TOK_LANE ? 1 : C::kCols / 2)] = fmul2(pack2f(q.x, q.y), ls);
+          sc[(2 * j + 1) % (TOK_LANE ? 1 : C::kCols / 2)] = fmul2(pack2f(q.z, q.w), ls);
         }
-        tc_wait_ld(v);
-        if (c + kChunk == C::kCols) {
-          // the accumulator (and the scales) go back before the last additions
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&ctl->acc_empty[buf]);
-            if (!TOK_LANE) mbar_arrive(&ctl->sc_empty[s]);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < kChunk / 2; ++j)
-          acc[c / 2 + j] = ffma2(pack2(v[2 * j], v[2 * j + 1]), TOK_LANE ? ls : sc[j], acc[c / 2 + j]);
       }
+#pragma unroll
+      for (int c = 0; c < C::kCols / kChunk; ++c) tc_wait_ld(v[c]);
+      // the accumulator and the scales go back before the additions
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&ctl->acc_empty[buf]);
+        if (!TOK_LANE) mbar_arrive(&ctl->sc_empty[s]);
+      }
+#pragma unroll
+      for (int c = 0; c < C::kCols / kChunk; ++c)
+#pragma unroll
+        for (int j = 0; j < kChunk / 2; ++j) {
+          const int at = c * (kChunk / 2) + j;
+          acc[at] = ffma2(pack2(v[c][2 * j], v[c][2 * j + 1]), sc[TOK_LANE ? 0 : at], acc[at]);
+        }
       if (!TOK_LANE && ++s == C::kScaleSlots) { s = 0; phase ^= 1u; }
       w0 = w1; w1 = w2; a0 = a1; a1 = a2;
     }

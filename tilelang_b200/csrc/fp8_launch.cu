@@ -1,6 +1,8 @@
 // Host side of the block-scaled fp8 products: shared-memory attributes once per device, cluster launches.
 #include "fp8_launch.h"
 
+#include <atomic>
+
 #include "fp8_gemm.cuh"
 #include "fp8_pair_gemm.cuh"
 
@@ -11,34 +13,67 @@ namespace {
 constexpr int kMaxDevices = 32;
 
 template <bool TOK_LANE, int TN>
-cudaError_t launch_tile(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const Fp8GemmParams& p, long long tiles,
-                        cudaStream_t stream) {
-  using C = Fp8TileConfig<TN>;
+cudaError_t prepare_tile(int* dev) {
   static bool attr_set[kMaxDevices] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  cudaError_t e = cudaGetDevice(dev);
   if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
-  auto kernel = fp8_tile_gemm_kernel<TOK_LANE, TN>;
-  if (!attr_set[dev]) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+  if (*dev < 0 || *dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  if (!attr_set[*dev]) {
+    e = cudaFuncSetAttribute(fp8_tile_gemm_kernel<TOK_LANE, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Fp8TileConfig<TN>::kSmemBytes);
     if (e != cudaSuccess) return e;
-    attr_set[dev] = true;
+    attr_set[*dev] = true;
   }
-  if (tiles * p.split > 0x7fffffffll) return cudaErrorInvalidValue;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.split));
-  cfg.blockDim = dim3(C::kThreads);
-  cfg.dynamicSmemBytes = C::kSmemBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  return cudaSuccess;
+}
+
+template <int TN>
+void tile_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, int split, long long ctas, cudaStream_t stream) {
+  *cfg = {};
+  cfg->gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg->blockDim = dim3(Fp8TileConfig<TN>::kThreads);
+  cfg->dynamicSmemBytes = Fp8TileConfig<TN>::kSmemBytes;
+  cfg->stream = stream;
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(p.split);
+  attr[0].val.clusterDim.x = static_cast<unsigned>(split);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, tmap_a, tmap_w, p);
+  cfg->attrs = attr;
+  cfg->numAttrs = 1;
+}
+
+template <bool TOK_LANE, int TN>
+cudaError_t launch_tile(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const Fp8GemmParams& p, long long tiles,
+                        cudaStream_t stream) {
+  int dev = 0;
+  const cudaError_t e = prepare_tile<TOK_LANE, TN>(&dev);
+  if (e != cudaSuccess) return e;
+  if (tiles * p.split > 0x7fffffffll) return cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[1];
+  tile_config<TN>(&cfg, attr, p.split, tiles * p.split, stream);
+  return cudaLaunchKernelEx(&cfg, fp8_tile_gemm_kernel<TOK_LANE, TN>, tmap_a, tmap_w, p);
+}
+
+// Clusters of every size that the device holds at once; a cluster lies within one group of SMs, so this is
+// less than the SMs divided by the size (148 SMs hold 144 single CTAs in clusters of 3 at best).
+template <bool TOK_LANE, int TN>
+cudaError_t resident_clusters(int split, int* clusters) {
+  static std::atomic<int> known[kMaxDevices][9] = {};
+  int dev = 0;
+  cudaError_t e = prepare_tile<TOK_LANE, TN>(&dev);
+  if (e != cudaSuccess) return e;
+  int n = known[dev][split].load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[1];
+    tile_config<TN>(&cfg, attr, split, split, nullptr);
+    e = cudaOccupancyMaxActiveClusters(&n, fp8_tile_gemm_kernel<TOK_LANE, TN>, &cfg);
+    if (e != cudaSuccess) return e;
+    known[dev][split].store(n, std::memory_order_relaxed);
+  }
+  *clusters = n;
+  return cudaSuccess;
 }
 
 }  // namespace
@@ -49,7 +84,16 @@ cudaError_t launch_fp8_tile_gemm(const CUtensorMap& tmap_a, const CUtensorMap& t
   switch (tile_tokens) {
     case 16: return launch_tile<false, 16>(tmap_a, tmap_w, p, tiles, stream);
     case 32: return launch_tile<false, 32>(tmap_a, tmap_w, p, tiles, stream);
-    case 64: return launch_tile<false, 64>(tmap_a, tmap_w, p, tiles, stream);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+cudaError_t fp8_resident_clusters(int tile_tokens, int split, int* clusters) {
+  if (split < 1 || split > 8) return cudaErrorInvalidValue;
+  switch (tile_tokens) {
+    case 16: return resident_clusters<false, 16>(split, clusters);
+    case 32: return resident_clusters<false, 32>(split, clusters);
+    case 128: return resident_clusters<true, 128>(split, clusters);
     default: return cudaErrorInvalidValue;
   }
 }

@@ -39,9 +39,12 @@ struct Fp8GemmParams {
 constexpr int kFp8BoxBytes = 128;   // columns of every box: one swizzle atom
 constexpr int kFp8BoxRows = 128;    // rows of a weight box, and of a token box whose tokens own lanes
 
-// Tokens own the accumulator's 128 lanes (tokens_on_lanes) or its columns, `tile_tokens` (16, 32, 64, 128) of them.
+// Tokens own the accumulator's 128 lanes (tokens_on_lanes) or its columns, `tile_tokens` (16, 32, 128) of them.
 cudaError_t launch_fp8_tile_gemm(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const Fp8GemmParams& p,
                                  bool tokens_on_lanes, int tile_tokens, long long tiles, cudaStream_t stream);
+
+// Clusters of `split` CTAs that the current device holds at once with this tile.
+cudaError_t fp8_resident_clusters(int tile_tokens, int split, int* clusters);
 
 // CTA pairs, 256 tokens x 256 columns (p.p_tiles counts tiles of p.tile_cols); `pairs` clusters of two. With
 // gate_codes the columns of a tile are 128 of the gate's and 128 of the up half's, and c (bf16) may be null.

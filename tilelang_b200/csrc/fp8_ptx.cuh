@@ -68,6 +68,9 @@ __device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[32]) {
   asm volatile("" : "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_32x32b_x16(taddr, r); }
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32b_x32(taddr, r); }
+
 // ---- clusters ----
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;

@@ -817,7 +817,7 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: Fp8Weight, trans_w: bool
     (N, K) :class:`Fp8Weight`; C is (M, N) in float16, bfloat16 or float32. With ``trans_w`` it is
     ``C = A @ W`` with ``a`` (M, N): the gradient of the input, (M, K), from the same weight.
     The two operands may be of different 8-bit types. Sums are float32 throughout, the result is rounded once.
-    ``token_tile`` (16, 32, 64, 128 or 256) and ``split`` (1 to 8) override the kernel's tile and the CTAs that
+    ``token_tile`` (16, 32, 128 or 256) and ``split`` (1 to 8) override the kernel's tile and the CTAs that
     share its contraction; 0 leaves them to the library."""
     args = _fp8_gemm_args("gemm_fp8", a, a_scale, w, trans_w, grouped=False)
     out = _fp8_gemm_out(a.shape[0], w.K if trans_w else w.N, out, out_dtype, a.device)
