@@ -31,6 +31,7 @@ _DTYPES = {
     "bfloat16": torch.bfloat16, "bf16": torch.bfloat16,
     "float32": torch.float32, "float": torch.float32, "fp32": torch.float32,
     "int8": torch.int8, "uint8": torch.uint8, "int32": torch.int32,
+    "float8_e4m3": torch.float8_e4m3fn, "float8_e4m3fn": torch.float8_e4m3fn, "float8_e5m2": torch.float8_e5m2,
 }
 
 
@@ -528,6 +529,87 @@ def bitnet_158_int8xint2_prefill(M: int, N: int, K: int, in_dtype="int8", out_dt
     (examples/bitnet-1.58b/kernel_benchmark/tilelang_bitnet_158_int8xint2_prefill.py:72-298)."""
     return _bitnet_factory("bitnet_158_int8xint2_prefill", M, N, K, in_dtype, out_dtype, accum_dtype, fast_decoding,
                            code_offset)
+
+
+# ---------------------------------------------------------------------------
+# 8-bit floating point with a scale for each block of 128
+# ---------------------------------------------------------------------------
+
+def matmul_fp8_block(M: int, N: int, K: int, in_dtype="float8_e4m3", out_dtype="bfloat16", accum_dtype="float32",
+                     weight_dtype: Any = None, block_size: int = 128, block_M=None, block_N=None, block_K=None,
+                     num_stages=None, threads=None, **ignored) -> DequantKernel:
+    """``C[M,N] = A @ B^T`` with both operands in 8-bit floating point: ``kernel(A, A_scale, B, B_scale)`` with A (M, K)
+    and one float32 scale for each row and 128 columns (``ops.quant_fp8``), B (N, K) and one for each block of
+    128 x 128 (``ops.quant_fp8_weight``). ``in_dtype`` and ``weight_dtype`` (the same unless given) are
+    "float8_e4m3" or "float8_e5m2"; ``out_dtype`` float16, bfloat16 or float32. The weight is read as it is."""
+    a_t, out_t = as_torch_dtype(in_dtype), as_torch_dtype(out_dtype)
+    w_t = a_t if weight_dtype is None else as_torch_dtype(weight_dtype)
+    if a_t not in ops._FP8_OF or w_t not in ops._FP8_OF:
+        raise ValueError("matmul_fp8_block: operands are float8_e4m3 or float8_e5m2")
+    if out_t not in ops._FLOAT_OF or as_torch_dtype(accum_dtype) != torch.float32:
+        raise ValueError("matmul_fp8_block: float16, bfloat16 or float32 output, float32 sums")
+    if block_size != 128:
+        raise ValueError("matmul_fp8_block: scales cover blocks of 128")
+    kb = ops._blocks128(K)
+    params = [Param("A", (M, K), a_t), Param("A_scale", (M, kb), torch.float32), Param("B", (N, K), w_t),
+              Param("B_scale", (ops._blocks128(N), kb), torch.float32), Param("C", (M, N), out_t)]
+
+    def impl(kernel: DequantKernel, A, A_scale, B, B_scale):
+        for t, p in zip((A, A_scale, B, B_scale), params):
+            _check(t, p)
+        return ops.gemm_fp8(A, A_scale, ops.Fp8Weight(B, B_scale), out_dtype=out_t)
+
+    return DequantKernel("matmul_fp8_block", params, [-1], impl, None,
+                         f"b200dq kind::f8f6f4 block-scaled: M={M} N={N} K={K} in={a_t} x {w_t} out={out_t}")
+
+
+class _Fp8Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, codes, scales, grad_dtype):
+        ctx.save_for_backward(codes, scales)
+        ctx.grad_dtype = grad_dtype
+        return ops.gemm_fp8(*ops.quant_fp8(x), ops.Fp8Weight(codes, scales), out_dtype=x.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d):
+        w = ops.Fp8Weight(*ctx.saved_tensors)
+        d_x = ops.gemm_fp8(*ops.quant_fp8(d.contiguous(), ctx.grad_dtype), w, trans_w=True, out_dtype=d.dtype)
+        return d_x, None, None, None
+
+
+class Fp8Linear(torch.nn.Module):
+    """A linear layer whose weight is kept in 8-bit floating point (:class:`ops.Fp8Weight`, (N, K)): the input is
+    quantised per row and 128 columns, multiplied, and the bias (if any) added in the output dtype, which is the
+    input's. Differentiable in the input (and bias); the weight is a constant. The incoming gradient is quantised
+    to ``grad_dtype`` and multiplied with the same weight bytes; the quantiser counts as the identity."""
+
+    def __init__(self, weight: "ops.Fp8Weight", bias: Optional[torch.Tensor] = None,
+                 grad_dtype: torch.dtype = torch.float8_e4m3fn):
+        super().__init__()
+        ops._check_fp8_target(grad_dtype)
+        if weight.codes.dim() != 2:
+            raise ValueError("Fp8Linear: one (N, K) weight")
+        self.weight, self.bias, self.grad_dtype = weight, bias, grad_dtype
+        self.in_features, self.out_features = weight.K, weight.N
+
+    @classmethod
+    def from_float(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                   dtype: torch.dtype = torch.float8_e4m3fn, **kwargs) -> "Fp8Linear":
+        """Quantise a floating-point (N, K) weight on the device."""
+        return cls(ops.quant_fp8_weight(weight.detach().contiguous(), dtype), bias, **kwargs)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        """x (..., K) float16/bfloat16/float32 -> (..., N)."""
+        if x.shape[-1] != self.in_features:
+            raise ValueError(f"Fp8Linear: expected {self.in_features} input features, got {x.shape[-1]}")
+        x2 = x.reshape(-1, self.in_features)
+        if x2.shape[0] > 1 and (x2.stride(1) != 1 or x2.stride(0) < self.in_features):
+            x2 = x2.contiguous()
+        out = _Fp8Linear.apply(x2, self.weight.codes, self.weight.scales, self.grad_dtype)
+        if self.bias is not None:
+            out = out + self.bias.to(out.dtype)
+        return out.reshape(*x.shape[:-1], self.out_features)
 
 
 class BitLinear(torch.nn.Module):

@@ -243,6 +243,11 @@ def dispatch_fp8(x: torch.Tensor, experts: torch.Tensor, num_experts: int,
     return codes, scales, _exchange_out(x.detach(), experts, num_experts, codes, scales, dtype)
 
 
+def combine_rows(y: torch.Tensor, row_of: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
+    """:func:`combine` from the (T, k) row indices alone."""
+    return combine(y, ExchangePlan(row_of, row_of.new_empty(0)), weights)
+
+
 def combine(y: torch.Tensor, plan: ExchangePlan, weights: torch.Tensor) -> torch.Tensor:
     """Back from expert order: ``out[t] = sum_s weights[t, s] * y[plan.row_of[t, s]]``, float32 sums in slot order
     rounded once to y's dtype; dropped pairs add nothing. ``y`` (T * k, H) contiguous float16, bfloat16 or float32,
@@ -253,6 +258,8 @@ def combine(y: torch.Tensor, plan: ExchangePlan, weights: torch.Tensor) -> torch
     row_of = plan.row_of
     if row_of.device != y.device or weights.device != y.device:
         raise ValueError("y, the plan and the weights must be on one device")
+    if row_of.dtype != torch.int64 or row_of.dim() != 2 or not row_of.is_contiguous():
+        raise ValueError("row indices must be a contiguous int64 tensor of shape (tokens, top_k)")
     if not weights.dtype.is_floating_point or weights.shape != row_of.shape:
         raise ValueError(f"weights must be floating point of shape {tuple(row_of.shape)}, got {weights.dtype} {tuple(weights.shape)}")
     if y.shape[0] != row_of.numel() or y.shape[1] == 0:
@@ -263,9 +270,91 @@ def combine(y: torch.Tensor, plan: ExchangePlan, weights: torch.Tensor) -> torch
     return _Combine.apply(y, row_of, weights)
 
 
+class _Fp8Mlp(torch.autograd.Function):
+    """The expert MLP on rows sorted by expert; gradient of the rows (the quantised weights are constants)."""
+
+    @staticmethod
+    def forward(ctx, x_sorted, counts, mlp, rows_behind):
+        codes, scales = ops.quant_fp8(x_sorted)
+        act, act_scales, h = ops.gemm_fp8_gated(codes, scales, mlp.w1, counts, keep_h=True)
+        y = ops.gemm_fp8_grouped(act, act_scales, mlp.w2, counts, out_dtype=x_sorted.dtype)
+        ctx.save_for_backward(h, counts, mlp.w1.codes, mlp.w1.scales, mlp.w2.codes, mlp.w2.scales)
+        ctx.grad_dtype, ctx.rows_behind = mlp.grad_dtype, rows_behind
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_y):
+        h, counts, *w = ctx.saved_tensors
+        w1, w2 = ops.Fp8Weight(*w[:2]), ops.Fp8Weight(*w[2:])
+        d_codes, d_scales = ops.quant_fp8(d_y.contiguous(), ctx.grad_dtype)
+        d_act = ops.gemm_fp8_grouped(d_codes, d_scales, w2, counts, trans_w=True, out_dtype=h.dtype)
+        d_codes, d_scales = ops.silu_mul_backward_quant_fp8(h, d_act, ctx.grad_dtype)
+        # the products do not write rows behind the last expert's
+        d_x = (torch.zeros if ctx.rows_behind else torch.empty)((h.shape[0], w1.K), dtype=d_y.dtype, device=h.device)
+        ops.gemm_fp8_grouped(d_codes, d_scales, w1, counts, trans_w=True, out=d_x)
+        return d_x, None, None, None
+
+
+class Fp8ExpertMLP(ExpertMLP):
+    """``y = W2( silu(g) * u )`` with ``[g, u] = W1(x)``, experts' weights in 8-bit floating point
+    (:class:`ops.Fp8Weight`: ``w1`` (E, 2F, H) with the gate's rows first, ``w2`` (E, H, F)), activations
+    quantised per row and 128 columns on their way: tokens by the dispatch, the gated intermediate by the
+    first product. Goes where :func:`make_gpu_expert_mlp`'s result goes (:func:`moe_forward`,
+    :func:`moe_forward_ep`).
+
+    Differentiable in the tokens and the routing weights; the experts' weights are constants. The gradient is
+    quantised like the activations, to ``grad_dtype``, and multiplied with the same weight bytes; the
+    quantiser itself counts as the identity."""
+
+    def __init__(self, w1: "ops.Fp8Weight", w2: "ops.Fp8Weight", grad_dtype: torch.dtype = torch.float8_e4m3fn):
+        ops._check_fp8_target(grad_dtype)
+        if w1.codes.dim() != 3 or w2.codes.dim() != 3:
+            raise ValueError("w1 and w2 hold one matrix per expert: codes of shape (E, 2F, H) and (E, H, F)")
+        if w1.num_groups != w2.num_groups or w1.N != 2 * w2.K or w1.K != w2.N:
+            raise ValueError(f"w1 {tuple(w1.codes.shape)} and w2 {tuple(w2.codes.shape)} are not (E, 2F, H) and (E, H, F)")
+        self.w1, self.w2, self.grad_dtype = w1, w2, grad_dtype
+        self.combine = combine_rows
+
+    def _check(self, x: torch.Tensor) -> None:
+        if x.dtype not in (torch.float16, torch.bfloat16) or x.dim() != 2 or x.shape[1] != self.w1.K:
+            raise ValueError(f"rows must be float16 or bfloat16 of width {self.w1.K}, got {x.dtype} {tuple(x.shape)}")
+
+    def __call__(self, x_sorted: torch.Tensor, counts) -> torch.Tensor:
+        """Rows sorted by expert -> rows. Rows behind the last expert's are undefined, their gradient is zero."""
+        self._check(x_sorted)
+        counts = ops._device_counts(counts, self.w1.num_groups, x_sorted.shape[0], x_sorted.device)
+        if torch.is_grad_enabled() and x_sorted.requires_grad:
+            return _Fp8Mlp.apply(x_sorted, counts, self, True)
+        return self._run(*ops.quant_fp8(x_sorted), counts, x_sorted.dtype)
+
+    def _run(self, codes, scales, counts, dtype):
+        act, act_scales = ops.gemm_fp8_gated(codes, scales, self.w1, counts)
+        return ops.gemm_fp8_grouped(act, act_scales, self.w2, counts, out_dtype=dtype)
+
+    def layer(self, x: torch.Tensor, experts: torch.Tensor, weights: torch.Tensor, num_experts: int) -> torch.Tensor:
+        """The layer behind the router: tokens (T, H), their experts and weights (T, k) -> (T, H)."""
+        if num_experts != self.w1.num_groups:
+            raise ValueError(f"the router has {num_experts} experts, the weights {self.w1.num_groups}")
+        self._check(x)
+        if torch.is_grad_enabled() and x.requires_grad:
+            rows, plan = dispatch(x, experts, num_experts)
+            # the dispatch's gradient reads no row behind the last expert's
+            return combine(_Fp8Mlp.apply(rows, plan.counts, self, False), plan, weights)
+        codes, scales, plan = dispatch_fp8(x, experts, num_experts)
+        return combine(self._run(codes, scales, plan.counts, x.dtype), plan, weights)
+
+
 def moe_forward(x: torch.Tensor, logits: torch.Tensor, top_k: int, num_experts: int, mlp: ExpertMLP) -> torch.Tensor:
     """Single-device MoE layer: route, gather rows by expert, expert MLP, weighted combine."""
     weights, experts = route(logits, top_k)
+    if isinstance(mlp, Fp8ExpertMLP):
+        return mlp.layer(x, experts, weights, num_experts)
+    if (x.is_cuda and x.dtype in ops._FLOAT_OF and num_experts <= 1024 and x.dim() == 2 and x.shape[1] > 0
+            and x.stride(1) == 1 and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1])):
+        # the same order of rows as below, in one to three launches instead of some ten
+        x_sorted, plan = dispatch(x, experts, num_experts)
+        return mlp.combine(mlp(x_sorted, plan.counts), plan.row_of, weights.contiguous())
     order, token_of_row, counts = sort_by_expert(experts, num_experts)
     x_sorted = x.index_select(0, token_of_row)
     # on a GPU the counts stay on the device: the grouped GEMMs plan their work there
