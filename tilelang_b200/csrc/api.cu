@@ -629,7 +629,19 @@ int run_gemm_fp8(const b200dq_fp8_gemm_args* a, const DeviceState* ds, cudaStrea
     p.gate_scales = a->gate_scales;
     p.ld_gate = a->ld_gate;
     p.gate_fp8 = a->gate_type;
-    CUDA_OK(launch_fp8_pair_gemm(tmap_a, tmap_w, p, static_cast<int>(std::min<long long>(plan.tiles, ds->sm_count / 2)), stream));
+    CUtensorMap tmap_c = tmap_a;                             // any valid map: not read unless c_vec16 is set
+    if (p.c_vec16 && a->c != nullptr) {
+      const int size = out_elem_size(a->out_type);
+      const cuuint64_t dims[2] = {static_cast<cuuint64_t>(outer), static_cast<cuuint64_t>(a->M)};
+      const cuuint64_t strides[1] = {static_cast<cuuint64_t>(outer) * size};
+      const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / size), 32}, estr[2] = {1, 1};
+      const CUtensorMapDataType type = a->out_type == OUT_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                       : a->out_type == OUT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+      const CUresult r = g_encode(&tmap_c, type, 2, a->c, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+      if (r != CUDA_SUCCESS) return fail("gemm_fp8: cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(r));
+    }
+    CUDA_OK(launch_fp8_pair_gemm(tmap_a, tmap_w, tmap_c, p, static_cast<int>(std::min<long long>(plan.tiles, ds->sm_count / 2)), stream));
     return 0;
   }
   CUDA_OK(launch_fp8_tile_gemm(tmap_a, tmap_w, p, plan.token_tile >= 128, plan.token_tile, plan.tiles, stream));

@@ -98,8 +98,8 @@ cudaError_t fp8_resident_clusters(int tile_tokens, int split, int* clusters) {
   }
 }
 
-cudaError_t launch_fp8_pair_gemm(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const Fp8GemmParams& p, int pairs,
-                                 cudaStream_t stream) {
+cudaError_t launch_fp8_pair_gemm(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const CUtensorMap& tmap_c,
+                                 const Fp8GemmParams& p, int pairs, cudaStream_t stream) {
   static_assert(kFp8PairMaxGroups == kPairMaxGroups, "tile table");
   static bool attr_set[kMaxDevices][2] = {};
   int dev = 0;
@@ -113,7 +113,7 @@ cudaError_t launch_fp8_pair_gemm(const CUtensorMap& tmap_a, const CUtensorMap& t
     if (e != cudaSuccess) return e;
     attr_set[dev][gated] = true;
   }
-  kernel<<<2 * pairs, kPairThreads, kPairSmemBytes, stream>>>(tmap_a, tmap_w, p);
+  kernel<<<2 * pairs, kPairThreads, kPairSmemBytes, stream>>>(tmap_a, tmap_w, tmap_c, p);
   return cudaGetLastError();
 }
 

@@ -31,10 +31,11 @@
 namespace b200dq {
 
 constexpr int kPairThreads = 384;
-constexpr int kPairStages = 6;
+constexpr int kPairStages = 5;
 constexpr int kPairHalf = 128 * 128;                          // one operand's half tile: 128 rows x 128 bytes
 constexpr int kPairStageBytes = 2 * kPairHalf;
-constexpr int kPairStageOut = 32 * 128;                       // a warp's output rows, 128 bytes each
+constexpr int kPairBoxBytes = 32 * 128;                       // 32 output rows of 128 bytes: one store box
+constexpr int kPairStageOut = 2 * kPairBoxBytes;              // a warp's staging
 constexpr int kPairStrip = 16;
 constexpr int kPairMaxGroups = 256;                           // groups whose tile table fits the control block
 // setmaxnreg moves registers from warps 0-3 to the eight summing warps: 128 * 40 + 256 * 232 = 384 * 168
@@ -112,19 +113,24 @@ __device__ __forceinline__ uint4 ld_shared4(uint32_t addr) {
   return v;
 }
 
-// 32 rows x 128 columns of fp32 sums (thread = row) to C, 128 bytes of each row at a time through the
-// warp's 4 KB of shared memory (16-byte chunks rotated by the row: no bank conflicts either way).
+// 32 rows x 128 columns of fp32 sums (thread = row) to C, 128 bytes of each row at a time through one of the
+// warp's two boxes in shared memory (16-byte chunks rotated by the row, as the tensor map's 128-byte
+// swizzle has them: no bank conflicts). Whole boxes leave by TMA, which reads them while the warp goes
+// on (moving the rows through registers again took three passes of the shared-memory pipe, 2450
+// cycles a tile); where a group ends inside the box, or C's rows do not start on 16 bytes, the warp writes.
 template <int OUT_TYPE>
-__device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, uint32_t stage, const uint64_t (&acc)[64],
-                                               long long m_first, int rows, int col0, int lane) {
+__device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, const CUtensorMap* tmap_c, uint32_t stage,
+                                               const uint64_t (&acc)[64], int m_first, int rows, int col0, int lane) {
   constexpr int kSize = OUT_TYPE == OUT_F32 ? 4 : 2;
   constexpr int kCols = 128 / kSize;                          // columns of a pass
-  const uint32_t out_at = stage + lane * 128, out_rot = (lane & 7) << 4;
-  const int chunk = lane & 7, row0 = lane >> 3;
-  const long long pitch = p.ldc * kSize;
-  uint8_t* dst = static_cast<uint8_t*>(p.c) + (m_first + row0) * pitch + (col0 + chunk * (16 / kSize)) * kSize;
+  const uint32_t out_rot = (lane & 7) << 4;
+  // a box may hang over the last row of C, which the hardware cuts off, but not over the last row of a group
+  const bool whole = p.c_vec16 && (rows == 32 || (rows > 0 && p.counts == nullptr));
 #pragma unroll
   for (int pass = 0; pass < 128 / kCols; ++pass) {
+    const uint32_t box = stage + (pass & 1) * kPairBoxBytes;
+    if (lane == 0) tma_store_wait_read<1>();                  // the copy before last has read this box
+    __syncwarp();
 #pragma unroll
     for (int j = 0; j < 8; ++j) {                             // 16-byte chunks of this thread's row
       uint32_t h[4];
@@ -138,37 +144,38 @@ __device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, uint32_t 
           h[i] = OUT_TYPE == OUT_BF16 ? bf162_as_u32(__floats2bfloat162_rn(f.x, f.y)) : h2_as_u32(__floats2half2_rn(f.x, f.y));
         }
       }
-      st_shared4(out_at + ((j << 4) ^ out_rot), h);
+      st_shared4(box + lane * 128 + ((j << 4) ^ out_rot), h);
     }
-    __syncwarp();
-    uint4 v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int row = i * 4 + row0;
-      v[i] = ld_shared4(stage + row * 128 + ((chunk ^ (row & 7)) << 4));
-    }
-    __syncwarp();
-    const int col = col0 + pass * kCols + chunk * (16 / kSize);
-    if (col < p.P) {
-      if (p.c_vec16) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i * 4 + row0 < rows) *reinterpret_cast<uint4*>(dst + i * 4 * pitch) = v[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (i * 4 + row0 >= rows) continue;
-          const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+    const int col = col0 + pass * kCols;
+    if (whole) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (col < p.P) tma_store_2d_at(tmap_c, box, col, m_first);
+        tma_store_commit();
+      }
+    } else {
+      __syncwarp();
+      const int chunk = lane & 7;
+      const int c = col + chunk * (16 / kSize);
+#pragma unroll 1
+      for (int row = lane >> 3; row < rows; row += 4) {
+        const uint4 v = ld_shared4(box + row * 128 + ((chunk ^ (row & 7)) << 4));
+        uint8_t* dst = static_cast<uint8_t*>(p.c) + (static_cast<size_t>(m_first + row) * p.ldc + c) * kSize;
+        if (p.c_vec16 && c < p.P) {
+          *reinterpret_cast<uint4*>(dst) = v;
+        } else {
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int e = 0; e < 16 / kSize; ++e) {
-            if (col + e >= p.P) break;
-            if (kSize == 4) reinterpret_cast<uint32_t*>(dst + i * 4 * pitch)[e] = w[e];
-            else reinterpret_cast<uint16_t*>(dst + i * 4 * pitch)[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+            if (c + e >= p.P) break;
+            if (kSize == 4) reinterpret_cast<uint32_t*>(dst)[e] = w[e];
+            else reinterpret_cast<uint16_t*>(dst)[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
           }
         }
       }
+      __syncwarp();
     }
-    dst += 128;
   }
 }
 
@@ -187,6 +194,8 @@ template <int FP8>
 __device__ __forceinline__ void fp8_pair_gate(const Fp8GemmParams& p, uint32_t mine, uint32_t other, const uint64_t (&acc)[64],
                                               int half, int quarter, long long m, bool in, int f0, int lane) {
   float act[64];
+  if (lane == 0) tma_store_wait_read<0>();                    // copies of the last tile's rows have left the boxes
+  __syncwarp();
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     // half 0 keeps columns 0-63 and sends 64-127, half 1 the other way round
@@ -244,7 +253,7 @@ __device__ __forceinline__ void fp8_pair_gate(const Fp8GemmParams& p, uint32_t m
 template <bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
-                     const Fp8GemmParams p) {
+                     const __grid_constant__ CUtensorMap tmap_c, const Fp8GemmParams p) {
   extern __shared__ __align__(1024) uint8_t fp8_pair_smem[];     // swizzle atoms start on 1 KiB boundaries
   uint8_t* smem = fp8_pair_smem;
   uint8_t* stage_out = smem + kPairStages * kPairStageBytes;
@@ -407,16 +416,17 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         else
           fp8_pair_gate<FP8_E5M2>(p, stage, other, acc, half, quarter, m_first + lane, in, done.p0, lane);
         if (ok && p.c != nullptr)
-          fp8_pair_store<OUT_BF16>(p, stage, acc, m_first, rows, done.p0 + half * (p.P / 2), lane);
+          fp8_pair_store<OUT_BF16>(p, &tmap_c, stage, acc, m_first, rows, done.p0 + half * (p.P / 2), lane);
       } else if (ok) {
         const int col0 = done.p0 + half * 128;
-        if (p.out_type == OUT_BF16) fp8_pair_store<OUT_BF16>(p, stage, acc, m_first, rows, col0, lane);
-        else if (p.out_type == OUT_F16) fp8_pair_store<OUT_F16>(p, stage, acc, m_first, rows, col0, lane);
-        else fp8_pair_store<OUT_F32>(p, stage, acc, m_first, rows, col0, lane);
+        if (p.out_type == OUT_BF16) fp8_pair_store<OUT_BF16>(p, &tmap_c, stage, acc, m_first, rows, col0, lane);
+        else if (p.out_type == OUT_F16) fp8_pair_store<OUT_F16>(p, &tmap_c, stage, acc, m_first, rows, col0, lane);
+        else fp8_pair_store<OUT_F32>(p, &tmap_c, stage, acc, m_first, rows, col0, lane);
       }
     }
   }
 
+  if (warp >= 4 && lane == 0) tma_store_wait_read<0>();       // copies have read their boxes before the memory goes away
   if (*abort_flag) {
     // copies in flight land before the shared memory goes away
     const uint64_t t0 = globaltimer_ns();

@@ -149,6 +149,13 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// tma_store_2d from a shared-memory address.
+__device__ __forceinline__ void tma_store_2d_at(const CUtensorMap* tmap, uint32_t smem_src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tmap), "r"(smem_src),
+               "r"(c0), "r"(c1)
+               : "memory");
+}
+
 // ---- asynchronous 4-byte copies ----
 __device__ __forceinline__ void cp_async4(uint32_t smem_dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_dst), "l"(src) : "memory");
