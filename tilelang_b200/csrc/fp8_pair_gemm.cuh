@@ -118,9 +118,11 @@ __device__ __forceinline__ uint4 ld_shared4(uint32_t addr) {
 // swizzle has them: no bank conflicts). Whole boxes leave by TMA, which reads them while the warp goes
 // on (moving the rows through registers again took three passes of the shared-memory pipe, 2450
 // cycles a tile); where a group ends inside the box, or C's rows do not start on 16 bytes, the warp writes.
+// `swap` = 64: the thread's first 64 columns are the tile's second 64 (gated u).
 template <int OUT_TYPE>
 __device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, const CUtensorMap* tmap_c, uint32_t stage,
-                                               const uint64_t (&acc)[64], int m_first, int rows, int col0, int lane) {
+                                               const uint64_t (&acc)[64], int m_first, int rows, int col0, int swap,
+                                               int lane) {
   constexpr int kSize = OUT_TYPE == OUT_F32 ? 4 : 2;
   constexpr int kCols = 128 / kSize;                          // columns of a pass
   const uint32_t out_rot = (lane & 7) << 4;
@@ -146,7 +148,7 @@ __device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, const CUt
       }
       st_shared4(box + lane * 128 + ((j << 4) ^ out_rot), h);
     }
-    const int col = col0 + pass * kCols;
+    const int col = col0 + ((pass * kCols) ^ swap);
     if (whole) {
       fence_proxy_async_smem();
       __syncwarp();
@@ -187,67 +189,85 @@ __device__ __forceinline__ void fp8_pair_add(uint64_t (&acc)[64], const int at, 
 
 __device__ __forceinline__ void pair_barrier(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
-// The two warps of a lane quarter: `half` 0 holds g, 1 holds u of 32 tokens x 128 features. Each sends
-// the half that the other one works on (32 columns at a time, 16-byte chunks rotated by the row), then
-// quantises its 64 features. `mine`, `other`: their 4 KB of shared memory.
-template <int FP8>
-__device__ __forceinline__ void fp8_pair_gate(const Fp8GemmParams& p, uint32_t mine, uint32_t other, const uint64_t (&acc)[64],
-                                              int half, int quarter, long long m, bool in, int f0, int lane) {
-  float act[64];
-  if (lane == 0) tma_store_wait_read<0>();                    // copies of the last tile's rows have left the boxes
-  __syncwarp();
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    // half 0 keeps columns 0-63 and sends 64-127, half 1 the other way round
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint64_t lo = half == 0 ? acc[32 + r * 16 + 2 * j] : acc[r * 16 + 2 * j];
-      const uint64_t hi = half == 0 ? acc[32 + r * 16 + 2 * j + 1] : acc[r * 16 + 2 * j + 1];
-      const float2 a = unpack2(lo), b = unpack2(hi);
-      const uint32_t w[4] = {__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y)};
-      st_shared4(mine + lane * 128 + ((j ^ (lane & 7)) << 4), w);
-    }
-    pair_barrier(1 + quarter);
-    uint4 in4[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) in4[j] = ld_shared4(other + lane * 128 + ((j ^ (lane & 7)) << 4));
-    pair_barrier(1 + quarter);                                // the partner may write again
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint4 o = in4[j];
-      const float2 a = unpack2(half == 0 ? acc[r * 16 + 2 * j] : acc[32 + r * 16 + 2 * j]);
-      const float2 b = unpack2(half == 0 ? acc[r * 16 + 2 * j + 1] : acc[32 + r * 16 + 2 * j + 1]);
-      const float own[4] = {a.x, a.y, b.x, b.y}, got[4] = {__uint_as_float(o.x), __uint_as_float(o.y), __uint_as_float(o.z), __uint_as_float(o.w)};
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        act[r * 32 + 4 * j + e] = half == 0 ? silu_mul_of(own[e], got[e]) : silu_mul_of(got[e], own[e]);
-    }
-  }
+// silu(g) u on two values at a time, as sigmoid_of and silu_mul_of round it.
+__device__ __forceinline__ uint64_t silu_mul2(uint64_t g, uint64_t u) {
+  const float2 t = unpack2(fmul2(g, pack2f(-1.4426950408889634f, -1.4426950408889634f)));
+  float2 e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+  const float2 d = unpack2(fadd2(pack2f(e.x, e.y), pack2f(1.0f, 1.0f)));
+  float2 r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(d.y));
+  return fmul2(fmul2(g, pack2f(r.x, r.y)), u);
+}
+
+// This warp's 64 features, in place of the first half of `acc`; returns the largest magnitude.
+template <bool GATE>
+__device__ __forceinline__ float fp8_pair_act(uint64_t (&acc)[64], uint32_t partner, int lane) {
   float amax = 0.f;
 #pragma unroll
-  for (int j = 0; j < 64; ++j) amax = max_magnitude(amax, act[j]);
-  asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + lane * 4), "f"(amax) : "memory");
+  for (int j = 0; j < 16; ++j) {
+    const uint4 o = ld_shared4(partner + (j >> 3) * kPairBoxBytes + lane * 128 + (((j & 7) ^ (lane & 7)) << 4));
+    const uint64_t got[2] = {pack2(o.x, o.y), pack2(o.z, o.w)};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint64_t own = acc[2 * j + e];
+      const uint64_t v = GATE ? silu_mul2(own, got[e]) : silu_mul2(got[e], own);
+      const float2 f = unpack2(v);
+      amax = max_magnitude(max_magnitude(amax, f.x), f.y);
+      acc[2 * j + e] = v;
+    }
+  }
+  return amax;
+}
+
+// The two warps of a lane quarter hold g and u of 32 tokens x 128 features, each its own 64 features in the
+// first half of `acc`. They swap the second halves, compute silu(g) u on 64 features each, agree
+// on the rows' maxima and write codes. `mine`, `partner`: the two warps' pairs of boxes.
+template <int FP8>
+__device__ __forceinline__ void fp8_pair_gate(const Fp8GemmParams& p, uint32_t mine, uint32_t partner, uint64_t (&acc)[64],
+                                              int half, int quarter, int m_first, int rows, int f0, int lane) {
+  if (lane == 0) tma_store_wait_read<0>();                    // copies of h have read the boxes
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const float2 a = unpack2(acc[32 + 2 * j]), b = unpack2(acc[32 + 2 * j + 1]);
+    const uint32_t w[4] = {__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y)};
+    st_shared4(mine + (j >> 3) * kPairBoxBytes + lane * 128 + (((j & 7) ^ (lane & 7)) << 4), w);
+  }
   pair_barrier(1 + quarter);
-  float partner;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(partner) : "r"(other + lane * 4) : "memory");
-  amax = max_magnitude(amax, partner);
-  pair_barrier(1 + quarter);                                  // read before the next tile's rows overwrite it
+  float amax = half == 0 ? fp8_pair_act<true>(acc, partner, lane) : fp8_pair_act<false>(acc, partner, lane);
+  pair_barrier(1 + quarter);                                  // both have read
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(mine + kPairBoxBytes + lane * 4), "f"(amax) : "memory");
+  pair_barrier(1 + quarter);
+  float other;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(partner + kPairBoxBytes + lane * 4) : "memory");
+  amax = max_magnitude(amax, other);
   const float s = fp8_scale_of<FP8>(__float_as_uint(amax));
   const float inv = __frcp_rn(s);
-  if (in) {
-    uint8_t* dst = p.gate_codes + m * p.ld_gate + f0 + half * 64;
+  const uint64_t inv2 = pack2f(inv, inv);
+  // codes: 64 bytes of each row through the first box, so that a store instruction writes 8 rows' 64 bytes
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t w[4];
+  for (int j = 0; j < 4; ++j) {
+    uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float* a = act + j * 16 + i * 4;
-        w[i] = fp8_pair<FP8>(__fmul_rn(a[0], inv), __fmul_rn(a[1], inv)) | (fp8_pair<FP8>(__fmul_rn(a[2], inv), __fmul_rn(a[3], inv)) << 16);
-      }
-      *reinterpret_cast<uint4*>(dst + j * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = unpack2(fmul2(acc[j * 8 + 2 * i], inv2)), b = unpack2(fmul2(acc[j * 8 + 2 * i + 1], inv2));
+      w[i] = fp8_pair<FP8>(a.x, a.y) | (fp8_pair<FP8>(b.x, b.y) << 16);
     }
-    if (half == 0) p.gate_scales[m * p.p_tiles + f0 / 128] = s;
+    st_shared4(mine + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), w);
   }
+  if (half == 0 && lane < rows) p.gate_scales[static_cast<long long>(m_first + lane) * p.p_tiles + f0 / 128] = s;
+  __syncwarp();
+  uint8_t* dst = p.gate_codes + static_cast<long long>(m_first) * p.ld_gate + f0 + half * 64 + (lane & 3) * 16;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = i * 8 + (lane >> 2);
+    const uint4 v = ld_shared4(mine + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4));
+    if (row < rows) *reinterpret_cast<uint4*>(dst + row * p.ld_gate) = v;
+  }
+  pair_barrier(1 + quarter);                                  // the partner has read the maxima; the boxes are free
 }
 
 template <bool GATED>
@@ -340,6 +360,8 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     const uint32_t stage = smem_u32(stage_out + (warp - 4) * kPairStageOut);
     const uint32_t other = smem_u32(stage_out + ((warp - 4) ^ 4) * kPairStageOut);
     const uint32_t empty_bar = cluster_map(smem_u32(&ctl->acc_empty[0]), 0);
+    // gated, the warps of u take their columns in the order 64-127, 0-63: every warp then keeps its first 64
+    const uint32_t swap = GATED && half == 1 ? 64 : 0;
     const uint32_t acc_addr = tmem_base + lane_addr + half * 128;
     uint32_t i = 0;
     bool ok = true;
@@ -369,8 +391,8 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       ok &= mbar_wait(&ctl->acc_full[i & 1u], (i >> 1) & 1u, abort_flag, st, 14);
       __syncwarp();
       tc_fence_after_sync();
-      tmem_ld_32x32b_x32(acc_addr + (i & 1u) * 256, v[0]);
-      tmem_ld_32x32b_x32(acc_addr + (i & 1u) * 256 + 32, v[1]);
+      tmem_ld_32x32b_x32(acc_addr + (i & 1u) * 256 + swap, v[0]);
+      tmem_ld_32x32b_x32(acc_addr + (i & 1u) * 256 + swap + 32, v[1]);
 #pragma unroll 1
       for (int kb = 0; kb < p.q_blocks; ++kb, ++i) {
         const uint32_t buf = i & 1u, addr = acc_addr + buf * 256, next = acc_addr + (buf ^ 1u) * 256;
@@ -385,9 +407,9 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         tc_wait_ld(v[0]);
         tc_wait_ld(v[1]);
         fp8_pair_add(acc, 0, v[0], scale);
-        tmem_ld_32x32b_x32(addr + 64, v[0]);
+        tmem_ld_32x32b_x32(addr + (64 - swap), v[0]);
         fp8_pair_add(acc, 16, v[1], scale);
-        tmem_ld_32x32b_x32(addr + 96, v[1]);
+        tmem_ld_32x32b_x32(addr + (96 - swap), v[1]);
         tc_wait_ld(v[0]);
         tc_wait_ld(v[1]);
         tc_fence_before_sync();
@@ -398,30 +420,28 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
           ok &= mbar_wait(&ctl->acc_full[buf ^ 1u], ((i + 1) >> 1) & 1u, abort_flag, st, 14);
           __syncwarp();
           tc_fence_after_sync();
-          tmem_ld_32x32b_x32(next, v[0]);
+          tmem_ld_32x32b_x32(next + swap, v[0]);
         }
         fp8_pair_add(acc, 48, v[1], scale);
-        if (more) tmem_ld_32x32b_x32(next + 32, v[1]);
+        if (more) tmem_ld_32x32b_x32(next + swap + 32, v[1]);
         a0 = a1; w0 = w1; a1 = a2; w1 = w2;
       }
       const Fp8Tile done = tile;
       if (t + pairs < tiles) begin(t + pairs);
       const int m_first = done.m0 + rank * 128 + quarter * 32;
-      const int rows = min(32, done.m_end - m_first);
+      ok = __all_sync(0xffffffffu, ok);                        // a wait that gave up: no lane writes
+      const int rows = ok ? min(32, done.m_end - m_first) : 0;
       if (GATED) {
+        if (p.c != nullptr)
+          fp8_pair_store<OUT_BF16>(p, &tmap_c, stage, acc, m_first, rows, done.p0 + half * (p.P / 2), swap, lane);
         // both warps of a quarter meet in here, whatever happened to either
-        const bool in = ok && lane < rows;
-        if (p.gate_fp8 == FP8_E4M3)
-          fp8_pair_gate<FP8_E4M3>(p, stage, other, acc, half, quarter, m_first + lane, in, done.p0, lane);
-        else
-          fp8_pair_gate<FP8_E5M2>(p, stage, other, acc, half, quarter, m_first + lane, in, done.p0, lane);
-        if (ok && p.c != nullptr)
-          fp8_pair_store<OUT_BF16>(p, &tmap_c, stage, acc, m_first, rows, done.p0 + half * (p.P / 2), lane);
-      } else if (ok) {
+        if (p.gate_fp8 == FP8_E4M3) fp8_pair_gate<FP8_E4M3>(p, stage, other, acc, half, quarter, m_first, rows, done.p0, lane);
+        else fp8_pair_gate<FP8_E5M2>(p, stage, other, acc, half, quarter, m_first, rows, done.p0, lane);
+      } else {
         const int col0 = done.p0 + half * 128;
-        if (p.out_type == OUT_BF16) fp8_pair_store<OUT_BF16>(p, &tmap_c, stage, acc, m_first, rows, col0, lane);
-        else if (p.out_type == OUT_F16) fp8_pair_store<OUT_F16>(p, &tmap_c, stage, acc, m_first, rows, col0, lane);
-        else fp8_pair_store<OUT_F32>(p, &tmap_c, stage, acc, m_first, rows, col0, lane);
+        if (p.out_type == OUT_BF16) fp8_pair_store<OUT_BF16>(p, &tmap_c, stage, acc, m_first, rows, col0, 0, lane);
+        else if (p.out_type == OUT_F16) fp8_pair_store<OUT_F16>(p, &tmap_c, stage, acc, m_first, rows, col0, 0, lane);
+        else fp8_pair_store<OUT_F32>(p, &tmap_c, stage, acc, m_first, rows, col0, 0, lane);
       }
     }
   }
