@@ -178,6 +178,8 @@ struct CopyMove {
 template <typename MOVE>
 __global__ void __launch_bounds__(256) exchange_dispatch_small_kernel(const ExchangeSortParams p,
                                                                       const ExchangeRowsParams r, int per) {
+  chain_next();
+  chain_wait();
   extern __shared__ int exchange_smem[];
   int* all = exchange_smem;                       // [E + 1] pairs of each expert, then their first rows
   int* next = exchange_smem + p.num_experts + 1;  // [E + 1] those before this CTA's pairs, then the next free row
@@ -207,6 +209,8 @@ __global__ void __launch_bounds__(256) exchange_dispatch_small_kernel(const Exch
 
 // ---- many pairs: count, place, move ---------------------------------------------------------------
 __global__ void __launch_bounds__(256) exchange_count_kernel(const ExchangeSortParams p, long long per) {
+  chain_next();
+  chain_wait();
   extern __shared__ int exchange_smem[];
   const int bins = p.num_experts + 1;
   const long long first = blockIdx.x * per, last = min(p.tokens * p.top_k, first + per);
@@ -221,6 +225,8 @@ __global__ void __launch_bounds__(256) exchange_count_kernel(const ExchangeSortP
 // cuts its chunk into one piece per warp, counts the pieces and lets every warp place its own.
 constexpr int kPlaceWarps = 8;
 __global__ void __launch_bounds__(kPlaceWarps * 32) exchange_place_kernel(const ExchangeSortParams p, long long per) {
+  chain_next();
+  chain_wait();
   extern __shared__ int exchange_smem[];
   const int bins = p.num_experts + 1;
   int* all = exchange_smem;                // [bins]
@@ -266,6 +272,8 @@ __global__ void __launch_bounds__(kPlaceWarps * 32) exchange_place_kernel(const 
 
 template <typename MOVE>
 __global__ void __launch_bounds__(256) exchange_move_kernel(const ExchangeSortParams p, const ExchangeRowsParams r) {
+  chain_next();
+  chain_wait();
   for (long long t = blockIdx.x; t < p.tokens; t += gridDim.x) MOVE::run(r, t, p.row_of + t * p.top_k, p.top_k);
 }
 
@@ -281,6 +289,8 @@ template <> __device__ __forceinline__ float exchange_round<float>(float v) { re
 // resident: 128 against 80 us for 16384 x 6 rows of 2048).
 template <typename T>
 __global__ void __launch_bounds__(256) exchange_sum_kernel(const ExchangeSumParams p) {
+  chain_next();
+  chain_wait();
   constexpr int V = 16 / sizeof(T);
   const T* y = static_cast<const T*>(p.y);
   for (long long t = blockIdx.x; t < p.tokens; t += gridDim.x) {
@@ -334,6 +344,8 @@ __global__ void __launch_bounds__(256) exchange_sum_kernel(const ExchangeSumPara
 // threads across the row and two barriers for every four slots, took 205 us where this takes 150).
 template <typename T>
 __global__ void __launch_bounds__(256) exchange_sum_grad_kernel(const ExchangeSumGradParams p) {
+  chain_next();
+  chain_wait();
   constexpr int V = 16 / sizeof(T);
   constexpr int kUnroll = 4;
   const int lane = threadIdx.x & 31;

@@ -16,16 +16,16 @@ cudaError_t dispatch(const ExchangeSortParams& s, const ExchangeRowsParams& r, c
   if (pairs <= kExchangeOneLaunchPairs) {
     const int per = static_cast<int>((s.tokens + 295) / 296);              // two CTAs an SM
     const int grid = static_cast<int>((s.tokens + per - 1) / per);
-    exchange_dispatch_small_kernel<MOVE><<<grid, 256, 2 * bins * sizeof(int), stream>>>(s, r, per);
-    return cudaGetLastError();
+    return chain_launch(exchange_dispatch_small_kernel<MOVE>, grid, 256, 2 * bins * sizeof(int), stream, 0, s, r, per);
   }
   const long long per = std::max<long long>(512, (pairs + kExchangeMaxChunks - 1) / kExchangeMaxChunks);
   const int chunks = static_cast<int>((pairs + per - 1) / per);
-  exchange_count_kernel<<<chunks, 256, bins * sizeof(int), stream>>>(s, per);
-  exchange_place_kernel<<<chunks, kPlaceWarps * 32, (kPlaceWarps + 2) * bins * sizeof(int), stream>>>(s, per);
+  cudaError_t e = chain_launch(exchange_count_kernel, chunks, 256, bins * sizeof(int), stream, 0, s, per);
+  if (e != cudaSuccess) return e;
+  e = chain_launch(exchange_place_kernel, chunks, kPlaceWarps * 32, (kPlaceWarps + 2) * bins * sizeof(int), stream, 0, s, per);
+  if (e != cudaSuccess) return e;
   const int grid = static_cast<int>(std::min<long long>(s.tokens, 148 * 32));
-  exchange_move_kernel<MOVE><<<grid, 256, 0, stream>>>(s, r);
-  return cudaGetLastError();
+  return chain_launch(exchange_move_kernel<MOVE>, grid, 256, 0, stream, 0, s, r);
 }
 
 template <typename T>
@@ -46,18 +46,14 @@ cudaError_t launch_exchange_sum(const ExchangeSumParams& p, cudaStream_t stream)
   const int items = p.vec ? p.width / (p.type == EXCHANGE_F32 ? 4 : 8) : p.width;
   const int threads = std::min(256, (items + 31) / 32 * 32);
   const int grid = static_cast<int>(std::min<long long>(p.tokens, 148 * 64));
-  if (p.type == EXCHANGE_F16) exchange_sum_kernel<__half><<<grid, threads, 0, stream>>>(p);
-  else if (p.type == EXCHANGE_BF16) exchange_sum_kernel<__nv_bfloat16><<<grid, threads, 0, stream>>>(p);
-  else exchange_sum_kernel<float><<<grid, threads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return chain_launch(p.type == EXCHANGE_F16 ? exchange_sum_kernel<__half> : p.type == EXCHANGE_BF16 ? exchange_sum_kernel<__nv_bfloat16> : exchange_sum_kernel<float>,
+                      grid, threads, 0, stream, 0, p);
 }
 
 cudaError_t launch_exchange_sum_grad(const ExchangeSumGradParams& p, cudaStream_t stream) {
   const int grid = static_cast<int>(std::min<long long>((p.tokens * p.top_k + 7) / 8, 148 * 64));
-  if (p.type == EXCHANGE_F16) exchange_sum_grad_kernel<__half><<<grid, 256, 0, stream>>>(p);
-  else if (p.type == EXCHANGE_BF16) exchange_sum_grad_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(p);
-  else exchange_sum_grad_kernel<float><<<grid, 256, 0, stream>>>(p);
-  return cudaGetLastError();
+  return chain_launch(p.type == EXCHANGE_F16 ? exchange_sum_grad_kernel<__half> : p.type == EXCHANGE_BF16 ? exchange_sum_grad_kernel<__nv_bfloat16> : exchange_sum_grad_kernel<float>,
+                      grid, 256, 0, stream, 0, p);
 }
 
 }  // namespace b200dq

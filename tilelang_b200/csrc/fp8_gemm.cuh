@@ -13,6 +13,7 @@
 // Grouped (mixture of experts): rows of `a` are sorted by group, the rows of each group counted on
 // the device; every CTA finds its own tile from the counts, so nothing is planned on the host.
 #pragma once
+#include "chain_launch.cuh"
 #include "fp8_launch.h"
 #include "fp8_ptx.cuh"
 #include "umma_gemm.cuh"   // OutType, packed-float bit casts
@@ -159,18 +160,20 @@ fp8_tile_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     tma_prefetch_desc(&tmap_a);
     tma_prefetch_desc(&tmap_w);
   }
+  if (warp == 3) {
+    tmem_alloc(&ctl->tmem_base, C::kTmemCols);
+    tmem_relinquish();
+  }
+  chain_wait();
   if (warp == 2) {
     Fp8Tile tile;
     const bool valid = fp8_find_tile<TN>(p, blockIdx.x / p.split, lane, &tile);
     if (lane == 0) { ctl->tile = tile; ctl->valid = valid; }
   }
-  if (warp == 3) {
-    tmem_alloc(&ctl->tmem_base, C::kTmemCols);
-    tmem_relinquish();
-  }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  chain_next();
   const uint32_t tmem_base = ctl->tmem_base;
   const Fp8Tile tile = ctl->tile;
   // A tile behind the last one: every CTA of the cluster finds the same and does nothing but the

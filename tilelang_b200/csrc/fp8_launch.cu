@@ -27,21 +27,6 @@ cudaError_t prepare_tile(int* dev) {
   return cudaSuccess;
 }
 
-template <int TN>
-void tile_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, int split, long long ctas, cudaStream_t stream) {
-  *cfg = {};
-  cfg->gridDim = dim3(static_cast<unsigned>(ctas));
-  cfg->blockDim = dim3(Fp8TileConfig<TN>::kThreads);
-  cfg->dynamicSmemBytes = Fp8TileConfig<TN>::kSmemBytes;
-  cfg->stream = stream;
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(split);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg->attrs = attr;
-  cfg->numAttrs = 1;
-}
-
 template <bool TOK_LANE, int TN>
 cudaError_t launch_tile(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const Fp8GemmParams& p, long long tiles,
                         cudaStream_t stream) {
@@ -49,10 +34,8 @@ cudaError_t launch_tile(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, co
   const cudaError_t e = prepare_tile<TOK_LANE, TN>(&dev);
   if (e != cudaSuccess) return e;
   if (tiles * p.split > 0x7fffffffll) return cudaErrorInvalidValue;
-  cudaLaunchConfig_t cfg;
-  cudaLaunchAttribute attr[1];
-  tile_config<TN>(&cfg, attr, p.split, tiles * p.split, stream);
-  return cudaLaunchKernelEx(&cfg, fp8_tile_gemm_kernel<TOK_LANE, TN>, tmap_a, tmap_w, p);
+  return chain_launch(fp8_tile_gemm_kernel<TOK_LANE, TN>, static_cast<unsigned>(tiles * p.split), Fp8TileConfig<TN>::kThreads,
+                      Fp8TileConfig<TN>::kSmemBytes, stream, static_cast<unsigned>(p.split), tmap_a, tmap_w, p);
 }
 
 // Clusters of every size that the device holds at once; a cluster lies within one group of SMs, so this is
@@ -65,9 +48,17 @@ cudaError_t resident_clusters(int split, int* clusters) {
   if (e != cudaSuccess) return e;
   int n = known[dev][split].load(std::memory_order_relaxed);
   if (n == 0) {
-    cudaLaunchConfig_t cfg;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(split));
+    cfg.blockDim = dim3(Fp8TileConfig<TN>::kThreads);
+    cfg.dynamicSmemBytes = Fp8TileConfig<TN>::kSmemBytes;
     cudaLaunchAttribute attr[1];
-    tile_config<TN>(&cfg, attr, split, split, nullptr);
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
     e = cudaOccupancyMaxActiveClusters(&n, fp8_tile_gemm_kernel<TOK_LANE, TN>, &cfg);
     if (e != cudaSuccess) return e;
     known[dev][split].store(n, std::memory_order_relaxed);
@@ -113,8 +104,7 @@ cudaError_t launch_fp8_pair_gemm(const CUtensorMap& tmap_a, const CUtensorMap& t
     if (e != cudaSuccess) return e;
     attr_set[dev][gated] = true;
   }
-  kernel<<<2 * pairs, kPairThreads, kPairSmemBytes, stream>>>(tmap_a, tmap_w, tmap_c, p);
-  return cudaGetLastError();
+  return chain_launch(kernel, 2 * pairs, kPairThreads, kPairSmemBytes, stream, 2, tmap_a, tmap_w, tmap_c, p);
 }
 
 }  // namespace b200dq

@@ -271,7 +271,7 @@ __device__ __forceinline__ void fp8_pair_gate(const Fp8GemmParams& p, uint32_t m
 }
 
 template <bool GATED>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+__global__ void __launch_bounds__(kPairThreads, 1)
 fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                      const __grid_constant__ CUtensorMap tmap_c, const Fp8GemmParams p) {
   extern __shared__ __align__(1024) uint8_t fp8_pair_smem[];     // swizzle atoms start on 1 KiB boundaries
@@ -291,15 +291,17 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     tma_prefetch_desc(&tmap_a);
     tma_prefetch_desc(&tmap_w);
   }
-  if (warp == 3 && p.counts != nullptr) fp8_pair_prefixes(p, ctl, lane);
   if (warp == 2) {
     tmem_alloc_pair(&ctl->tmem_base, 512);
     tmem_relinquish_pair();
   }
+  chain_wait();
+  if (warp == 3 && p.counts != nullptr) fp8_pair_prefixes(p, ctl, lane);
   __syncwarp();
   tc_fence_before_sync();
   cluster_sync_all();                                         // the peer's barriers exist
   tc_fence_after_sync();
+  chain_next();
   const uint32_t tmem_base = ctl->tmem_base;
   const int token_tiles = p.counts != nullptr ? ctl->tile_prefix[p.num_groups] : (p.M + 255) / 256;
   const int tiles = token_tiles * p.p_tiles;

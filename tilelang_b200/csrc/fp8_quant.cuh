@@ -20,6 +20,7 @@
 
 #include <cstdint>
 
+#include "chain_launch.cuh"
 #include "fp8_quant_launch.h"
 
 namespace b200dq {
@@ -109,6 +110,8 @@ __device__ __forceinline__ uint4 quant16(const float (&v)[16], float* scale) {
 // gradient half a multiple of 128, and 16-byte aligned rows; the other kernel takes the rest.
 template <typename T, int OUT, int MODE>
 __global__ void __launch_bounds__(256) fp8_quant_vec_kernel(const Fp8QuantParams p) {
+  chain_next();
+  chain_wait();
   const int cols = MODE == FP8_OF_SILU_MUL_GRAD ? p.half : p.cols;
   const unsigned blocks = (cols + 127) / 128;            // blocks of a row (of one half of it for the gradient)
   const long long idx = blockIdx.x * 256ll + threadIdx.x;
@@ -175,6 +178,8 @@ __device__ __forceinline__ float fp8_source(const Fp8QuantParams& p, long long r
 // that loads and byte stores of a warp are contiguous.
 template <typename T, int OUT, int MODE>
 __global__ void __launch_bounds__(256) fp8_quant_any_kernel(const Fp8QuantParams p) {
+  chain_next();
+  chain_wait();
   const int lane = threadIdx.x & 31;
   const int blocks = (p.cols + 127) / 128;
   const long long idx = blockIdx.x * 8ll + (threadIdx.x >> 5);

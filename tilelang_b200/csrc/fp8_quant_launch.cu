@@ -12,11 +12,8 @@ cudaError_t launch(const Fp8QuantParams& p, cudaStream_t stream) {
   const long long row_blocks = ((MODE == FP8_OF_SILU_MUL_GRAD && p.vec ? p.half : p.cols) + 127) / 128;
   const long long grid = p.vec ? (p.rows * row_blocks * 8 + 255) / 256 : (p.rows * row_blocks + 7) / 8;
   if (grid > 0x7fffffffll) return cudaErrorInvalidValue;
-  if (p.vec)
-    fp8_quant_vec_kernel<T, OUT, MODE><<<static_cast<unsigned>(grid), 256, 0, stream>>>(p);
-  else
-    fp8_quant_any_kernel<T, OUT, MODE><<<static_cast<unsigned>(grid), 256, 0, stream>>>(p);
-  return cudaGetLastError();
+  return chain_launch(p.vec ? fp8_quant_vec_kernel<T, OUT, MODE> : fp8_quant_any_kernel<T, OUT, MODE>,
+                      static_cast<unsigned>(grid), 256, 0, stream, 0, p);
 }
 
 template <typename T, int OUT>
