@@ -327,8 +327,8 @@ int b200dq_exchange_dispatch(const void* experts, int32_t experts_int64, int64_t
                              int64_t ld_out, float* scales, int32_t fp8_type, int64_t* row_of, int64_t* counts,
                              void* scratch, size_t scratch_bytes, void* cuda_stream);
 
-/* out[t] = sum over s of weights[t, s] * y[row_of[t, s]] (weights NULL: all one; negative row_of: no
- * term), fp32 sums in slot order, one rounding. Also the gradient of the copying dispatch. */
+/* out[t] = sum over s of weights[t, s] * y[row_of[t, s]] (weights NULL: all one; a row_of outside
+ * [0, tokens * top_k): no term), fp32 sums in slot order, one rounding. Also the gradient of the copying dispatch. */
 int b200dq_exchange_sum(const void* y, const int64_t* row_of, const float* weights, void* out, int64_t tokens,
                         int32_t top_k, int32_t width, int32_t type, void* cuda_stream);
 

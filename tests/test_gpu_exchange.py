@@ -164,6 +164,20 @@ def test_only_the_gradients_that_are_asked_for():
     assert torch.equal(y.grad, torch.autograd.grad(moe.combine(y, plan, w.detach().half().float()), y, torch.ones_like(d))[0])
 
 
+def test_rows_outside_the_tensor_are_not_followed():
+    """Indices that no dispatch gives add nothing; in the backward pass they are neither read nor written."""
+    y = randn(12, 40, seed=1).requires_grad_()
+    row_of = torch.tensor([[0, 5], [12, 3], [2 ** 40, -1], [7, -2 ** 50], [1, 2], [-13, 4]], device=DEV)
+    w = torch.ones(6, 2, device=DEV).requires_grad_()
+    plan = moe.ExchangePlan(row_of, torch.zeros(1, dtype=torch.int64, device=DEV))
+    out = moe.combine(y, plan, w)
+    kept = (row_of >= 0) & (row_of < 12)
+    want = torch.where(kept.unsqueeze(-1), y.detach()[row_of.clamp(0, 11)], 0.0).sum(1)
+    assert torch.equal(out.detach(), want)
+    d_w, = torch.autograd.grad(out, w, torch.ones_like(out))
+    assert (d_w[~kept] == 0).all() and (d_w[kept] != 0).all()
+
+
 def test_two_captured_graphs_share_nothing():
     experts = [pick(2000, 4, 16, 1), pick(2000, 4, 16, 2)]
     x = randn(2000, 64, seed=3, dtype=torch.bfloat16)

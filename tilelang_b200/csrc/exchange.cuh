@@ -294,6 +294,7 @@ __global__ void __launch_bounds__(256) exchange_sum_kernel(const ExchangeSumPara
   chain_wait();
   constexpr int V = 16 / sizeof(T);
   const T* y = static_cast<const T*>(p.y);
+  const long long all_rows = p.tokens * p.top_k;          // indices outside add nothing and are not followed
   for (long long t = blockIdx.x; t < p.tokens; t += gridDim.x) {
     const long long* rows = p.row_of + t * p.top_k;
     const float* w = p.weights != nullptr ? p.weights + t * p.top_k : nullptr;
@@ -310,7 +311,7 @@ __global__ void __launch_bounds__(256) exchange_sum_kernel(const ExchangeSumPara
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
             const long long row = s0 + s < p.top_k ? rows[s0 + s] : -1;
-            kept[s] = row >= 0;
+            kept[s] = row >= 0 && row < all_rows;
             f[s] = kept[s] && w != nullptr ? w[s0 + s] : 1.f;
             if (kept[s]) v[s] = __ldcs(reinterpret_cast<const uint4*>(y + row * p.width) + c);
           }
@@ -332,7 +333,8 @@ __global__ void __launch_bounds__(256) exchange_sum_kernel(const ExchangeSumPara
       for (int c = threadIdx.x; c < p.width; c += blockDim.x) {
         float acc = 0.f;
         for (int s = 0; s < p.top_k; ++s)
-          if (rows[s] >= 0) acc = fmaf(w != nullptr ? w[s] : 1.f, Fp8In<T>::get(y[rows[s] * p.width + c]), acc);
+          if (rows[s] >= 0 && rows[s] < all_rows)
+            acc = fmaf(w != nullptr ? w[s] : 1.f, Fp8In<T>::get(y[rows[s] * p.width + c]), acc);
         out[c] = exchange_round<T>(acc);
       }
     }
@@ -353,11 +355,12 @@ __global__ void __launch_bounds__(256) exchange_sum_grad_kernel(const ExchangeSu
   const long long pairs = p.tokens * p.top_k;
   for (long long i = blockIdx.x * 8ll + (threadIdx.x >> 5); i < pairs; i += gridDim.x * 8ll) {
     const long long row = p.row_of[i];
-    const bool kept = row >= 0;
+    const bool kept = row >= 0 && row < pairs;
+    const long long at = row >= 0 ? row : -1 - row;
     const float w = kept ? p.weights[i] : 0.f;
     const T* d = static_cast<const T*>(p.d_out) + i / p.top_k * p.width;
     const T* y = p.d_weights != nullptr && kept ? static_cast<const T*>(p.y) + row * p.width : nullptr;
-    T* d_y = p.d_y != nullptr ? static_cast<T*>(p.d_y) + (kept ? row : -1 - row) * p.width : nullptr;
+    T* d_y = p.d_y != nullptr && at < pairs ? static_cast<T*>(p.d_y) + at * p.width : nullptr;
     float dot = 0.f;
     if (p.vec) {
       const int vecs = p.width / V;

@@ -592,8 +592,8 @@ _FP8_OF = {torch.float8_e4m3fn: _lib.FP8_E4M3, torch.float8_e5m2: _lib.FP8_E5M2}
 _FLOAT_OF = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # absent from builds without CUDA
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def _call(fn, what: str, device: torch.device, *args) -> None:
@@ -627,6 +627,8 @@ def _check_rows(name: str, t: torch.Tensor, device: Optional[torch.device] = Non
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
     rows, cols = t.shape
+    if rows >= 1 << 31 or cols >= 1 << 31:
+        raise ValueError(f"{name} has a side of 2^31 or more: {tuple(t.shape)}")
     if cols > 1 and t.stride(1) != 1:
         raise ValueError(f"{name} must have contiguous rows")
     if rows > 1 and t.stride(0) < cols:
