@@ -150,8 +150,8 @@ def _exchange_out(x: torch.Tensor, experts: torch.Tensor, num_experts: int, out:
     """Sorts the pairs and moves the rows of ``x`` into ``out``, on the current stream."""
     lib = _lib.load()
     T, k = experts.shape
-    plan = ExchangePlan(torch.empty((T, k), dtype=torch.int64, device=x.device),
-                        torch.empty(num_experts, dtype=torch.int64, device=x.device))
+    plan = ExchangePlan(ops._new(T, k, torch.int64, x.device),
+                        torch.empty_strided((num_experts,), (1,), dtype=torch.int64, device=x.device))
     if T == 0:
         plan.counts.zero_()
         return plan
@@ -187,7 +187,7 @@ class _Dispatch(torch.autograd.Function):
 
 def _exchange_sum(y: torch.Tensor, row_of: torch.Tensor, weights: Optional[torch.Tensor]) -> torch.Tensor:
     T, k = row_of.shape
-    out = torch.empty((T, y.shape[1]), dtype=y.dtype, device=y.device)
+    out = ops._new(T, y.shape[1], y.dtype, y.device)
     if T:
         ops._call(_lib.load().b200dq_exchange_sum, "b200dq_exchange_sum", y.device, y.data_ptr(), row_of.data_ptr(),
                   weights.data_ptr() if weights is not None else None, out.data_ptr(), T, k, y.shape[1],
@@ -226,7 +226,7 @@ def dispatch(x: torch.Tensor, experts: torch.Tensor, num_experts: int) -> Tuple[
     if torch.is_grad_enabled() and x.requires_grad:
         rows, row_of, counts = _Dispatch.apply(x, experts, num_experts)
         return rows, ExchangePlan(row_of, counts)
-    rows = torch.empty((experts.numel(), x.shape[1]), dtype=x.dtype, device=x.device)
+    rows = ops._new(experts.numel(), x.shape[1], x.dtype, x.device)
     return rows, _exchange_out(x, experts, num_experts, rows, None, None)
 
 
@@ -239,7 +239,7 @@ def dispatch_fp8(x: torch.Tensor, experts: torch.Tensor, num_experts: int,
     experts = _check_experts(x, experts, num_experts)
     rows = experts.numel()
     codes = ops._fp8_rows(rows, x.shape[1], dtype, x.device)
-    scales = torch.empty((rows, ops._blocks128(x.shape[1])), dtype=torch.float32, device=x.device)
+    scales = ops._new(rows, ops._blocks128(x.shape[1]), torch.float32, x.device)
     return codes, scales, _exchange_out(x.detach(), experts, num_experts, codes, scales, dtype)
 
 

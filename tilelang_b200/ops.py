@@ -638,9 +638,12 @@ def _check_rows(name: str, t: torch.Tensor, device: Optional[torch.device] = Non
 
 def _fp8_rows(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
     """(rows, cols) codes whose row pitch is a multiple of 16 bytes, as the products read them."""
-    if cols % 16 == 0:
-        return torch.empty((rows, cols), dtype=dtype, device=device)
-    return torch.empty((rows, (cols + 15) // 16 * 16), dtype=dtype, device=device)[:, :cols]
+    return torch.empty_strided((rows, cols), ((cols + 15) // 16 * 16, 1), dtype=dtype, device=device)
+
+
+def _new(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """A contiguous matrix (empty_strided takes two thirds of empty's time)."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
 
 
 def _check_fp8_target(dtype: torch.dtype) -> None:
@@ -667,7 +670,7 @@ def _quant_fp8(mode: int, what: str, x: torch.Tensor, d: Optional[torch.Tensor],
             raise ValueError(f"d must be {x.dtype} of shape {(rows, cols)}, got {d.dtype} {tuple(d.shape)}")
     out_cols = 2 * cols if mode == _lib.FP8_OF_SILU_MUL_GRAD else cols
     codes = _fp8_rows(rows, out_cols, dtype, x.device)
-    scales = torch.empty((rows, _blocks128(out_cols)), dtype=torch.float32, device=x.device)
+    scales = _new(rows, _blocks128(out_cols), torch.float32, x.device)
     if rows:
         _call(lib.b200dq_quant_fp8, what, x.device, mode, x.data_ptr(), ld_x, d.data_ptr() if d is not None else None,
               ld_d, codes.data_ptr(), codes.stride(0), scales.data_ptr(), rows, cols, _FLOAT_OF[x.dtype], _FP8_OF[dtype])
@@ -750,7 +753,8 @@ def _fp8_gemm_args(what: str, a: torch.Tensor, a_scale: torch.Tensor, w: Fp8Weig
     """Checks the operands of a product and fills the argument struct but for the output and the counts."""
     lda = _check_rows("a", a)
     dev = a.device
-    if a.dtype not in _FP8_OF:
+    a_type = _FP8_OF.get(a.dtype)
+    if a_type is None:
         raise TypeError(f"a must be float8_e4m3fn or float8_e5m2, got {a.dtype}")
     codes, scales = w.codes, w.scales
     for name, t in (("w.codes", codes), ("w.scales", scales)):
@@ -758,46 +762,48 @@ def _fp8_gemm_args(what: str, a: torch.Tensor, a_scale: torch.Tensor, w: Fp8Weig
             raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
         if t.device != dev:
             raise ValueError(f"{name} is on {t.device}, a on {dev}")
-    if codes.dtype not in _FP8_OF:
+    w_type = _FP8_OF.get(codes.dtype)
+    if w_type is None:
         raise TypeError(f"w.codes must be float8_e4m3fn or float8_e5m2, got {codes.dtype}")
-    if codes.dim() != (3 if grouped else 2):
-        raise ValueError(f"{what} takes w.codes of shape {'(E, N, K)' if grouped else '(N, K)'}, got {tuple(codes.shape)}")
-    N, K = codes.shape[-2:]
-    G = codes.shape[0] if grouped else 0
-    if N == 0 or K == 0 or (grouped and G == 0):
-        raise ValueError("w must not be empty")
+    shape, stride = codes.shape, codes.stride()
+    if len(shape) != (3 if grouped else 2):
+        raise ValueError(f"{what} takes w.codes of shape {'(E, N, K)' if grouped else '(N, K)'}, got {tuple(shape)}")
+    N, K = shape[-2], shape[-1]
+    G = shape[0] if grouped else 0
+    if N == 0 or K == 0 or (grouped and G == 0) or N >= 1 << 31 or K >= 1 << 31:
+        raise ValueError(f"w must not be empty, and its sides below 2^31, got {tuple(shape)}")
     inner = N if trans_w else K
-    M = a.shape[0]
-    if a.shape[1] != inner:
+    M, cols = a.shape
+    if cols != inner:
         raise ValueError(f"a must have shape (M, {inner}), got {tuple(a.shape)}")
-    if K > 1 and codes.stride(-1) != 1:
+    if K > 1 and stride[-1] != 1:
         raise ValueError("w.codes must have contiguous rows")
-    ldw = codes.stride(-2) if N > 1 else (K + 15) // 16 * 16
-    group_stride = codes.stride(0) if G > 1 else ldw * N
+    ldw = stride[-2] if N > 1 else (K + 15) // 16 * 16
+    group_stride = stride[0] if G > 1 else ldw * N
     if M == 1:
         lda = (inner + 15) // 16 * 16
-    if a.data_ptr() % 16 or lda % 16 or codes.data_ptr() % 16 or ldw % 16 or group_stride % 16:
+    a_ptr, w_ptr = a.data_ptr(), codes.data_ptr()
+    if (a_ptr | lda | w_ptr | ldw | group_stride) % 16:
         raise ValueError("rows of a and w.codes must start on 16-byte boundaries (quant_fp8 and quant_fp8_weight lay them out so)")
     if ldw < K or group_stride < ldw * N:
         raise ValueError("w.codes has rows or matrices that overlap")
     blocks = (_blocks128(N), _blocks128(K))
     want = (G, *blocks) if grouped else blocks
-    if scales.dtype != torch.float32 or tuple(scales.shape) != want or not scales.is_contiguous():
+    if scales.dtype != torch.float32 or scales.shape != want or not scales.is_contiguous():
         raise ValueError(f"w.scales must be contiguous float32 of shape {want}, got {scales.dtype} {tuple(scales.shape)}")
     ld_scale = _check_rows("a_scale", a_scale, dev)
-    if a_scale.dtype != torch.float32 or tuple(a_scale.shape) != (M, _blocks128(inner)):
+    if a_scale.dtype != torch.float32 or a_scale.shape != (M, _blocks128(inner)):
         raise ValueError(f"a_scale must be float32 of shape {(M, _blocks128(inner))}, got {a_scale.dtype} {tuple(a_scale.shape)}")
     # in the order of the struct: a, a_scale, w, w_scale, c, counts, pitches, sizes, groups, types
-    return _lib.Fp8GemmArgs(a.data_ptr(), a_scale.data_ptr(), codes.data_ptr(), scales.data_ptr(), None, None,
-                            lda, ld_scale, ldw, group_stride, M, N, K, G, 0, _FP8_OF[a.dtype], _FP8_OF[codes.dtype],
-                            0, 1 if trans_w else 0)
+    return _lib.Fp8GemmArgs(a_ptr, a_scale.data_ptr(), w_ptr, scales.data_ptr(), None, None, lda, ld_scale, ldw,
+                            group_stride, M, N, K, G, 0, a_type, w_type, 0, 1 if trans_w else 0)
 
 
 def _fp8_gemm_out(M: int, cols: int, out: Optional[torch.Tensor], out_dtype: torch.dtype, device: torch.device):
     if out is None:
         if out_dtype not in _FLOAT_OF:
             raise TypeError(f"out_dtype must be float16, bfloat16 or float32, not {out_dtype}")
-        return torch.empty((M, cols), dtype=out_dtype, device=device)
+        return _new(M, cols, out_dtype, device)
     _check_cuda_contig("out", out, device)
     if tuple(out.shape) != (M, cols) or out.dtype not in _FLOAT_OF:
         raise ValueError(f"out must be float16, bfloat16 or float32 of shape {(M, cols)}, got {out.dtype} {tuple(out.shape)}")
@@ -875,12 +881,12 @@ def gemm_fp8_gated(a: torch.Tensor, a_scale: torch.Tensor, w: Fp8Weight, counts=
         args.counts, args.counts_int64 = counts.data_ptr(), 1 if counts.dtype == torch.int64 else 0
     _ensure_init(dev)
     if not lib.b200dq_fp8_gated_fuses(M, w.N, w.K, w.num_groups):
-        h = _run_gemm_fp8(args, torch.empty((M, w.N), dtype=torch.float32, device=dev), "b200dq_gemm_fp8")
+        h = _run_gemm_fp8(args, _new(M, w.N, torch.float32, dev), "b200dq_gemm_fp8")
         codes, scales = silu_mul_quant_fp8(h, dtype)
         return (codes, scales, h.to(torch.bfloat16)) if keep_h else (codes, scales)
     codes = _fp8_rows(M, F, dtype, dev)
-    scales = torch.empty((M, _blocks128(F)), dtype=torch.float32, device=dev)
-    h = torch.empty((M, w.N), dtype=torch.bfloat16, device=dev) if keep_h else None
+    scales = _new(M, _blocks128(F), torch.float32, dev)
+    h = _new(M, w.N, torch.bfloat16, dev) if keep_h else None
     args.c, args.out_type = h.data_ptr() if keep_h else None, _lib.OUT_BF16
     args.gate_codes, args.gate_scales, args.ld_gate = codes.data_ptr(), scales.data_ptr(), codes.stride(0)
     args.gate_type = _FP8_OF[dtype]
