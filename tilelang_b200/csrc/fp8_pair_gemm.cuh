@@ -6,18 +6,20 @@
 // one of two accumulators that fill tensor memory, and eight warps move them, scaled, to fp32
 // registers: thread = one token, 128 columns, one scale per block; 64 packed fmas.
 //
-// What bounds it (4096 x 28672 x 8192, 826 us, 2330 TFLOP/s, the GPU at its power limit near 1.55 GHz): the
-// hand-over of accumulators. With the summing warps reduced to the barriers alone it takes 695 us, without
-// waiting for them 618 us. Two accumulators are all that tensor memory holds at this width; four of
-// 128 columns (twice the instructions, each half as wide) measured 932 us. So everything on the way round
+// What bounds it (4096 x 28672 x 8192, 772 us in a burst, 2490 TFLOP/s, the GPU at its power limit near 1.5 GHz): the
+// way round of an accumulator. Timestamps of one buffer, in cycles: hand-back seen to accumulator full 910
+// (four instructions of 128, issue, commit), first columns in registers 300, the rest read and added
+// 270, hand-back to the issuing warp 90; two buffers in turn make 780 a block, where the multiplication alone
+// needs 512 (590 at the rate it reaches with nobody waiting: 618 us). Tensor memory holds no third
+// accumulator of this width; four of 128 columns (twice the instructions, each half as wide) measured
+// 932 us, sixteen summing warps 957, three pieces in flight (registers spill) 839. So everything on the way
 // is short: the issuing warp runs uniformly (operands in uniform registers; a single issuing thread took
-// 920 us), commits the accumulator before the stage, and the summing warps hand back after
-// half of their additions. Strips of 16 token tiles: 826 us, 8: 840, 4: 868.
+// 920 us) and commits the accumulator before the stage. Strips of 16 token tiles, not 8: 826 against 840 us.
 //
 // Persistent: one pair per two SMs, tiles in strips of 16 token tiles so that the tiles in flight
 // share their operands in L2. warp 0: TMA producer (both CTAs); warp 1: MMA issuer (first CTA);
-// warps 2, 3: tensor memory, tile table; warps 4-11: sums and output. Finished rows go through 4 KB of
-// shared memory per warp, so that a store instruction writes whole 128-byte pieces.
+// warps 2, 3: tensor memory, tile table; warps 4-11: sums and output, which leaves through 8 KB of shared
+// memory per warp by TMA.
 //
 // GATED: weights are [gate; up], F rows each; the first CTA loads 128 gate rows, the second the 128 up
 // rows that belong to them, so that a tile's columns 0-127 and 128-255 are g and u of the same 128
@@ -387,14 +389,14 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       uint64_t acc[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) acc[j] = 0;
-      // Two pieces of 32 columns are in registers or on their way at any time; the order hands the accumulator
-      // back after half of the additions and fetches the next block's first half under the other half.
+      // Pieces of 32 columns, one being added while the next is read: under the multiplication a piece takes
+      // about 90 cycles to read and 64 to add (two warps share the pipes). The accumulator goes back with the
+      // last piece in registers.
       uint32_t v[2][32];
       ok &= mbar_wait(&ctl->acc_full[i & 1u], (i >> 1) & 1u, abort_flag, st, 14);
       __syncwarp();
       tc_fence_after_sync();
       tmem_ld_32x32b_x32(acc_addr + (i & 1u) * 256 + swap, v[0]);
-      tmem_ld_32x32b_x32(acc_addr + (i & 1u) * 256 + swap + 32, v[1]);
 #pragma unroll 1
       for (int kb = 0; kb < p.q_blocks; ++kb, ++i) {
         const uint32_t buf = i & 1u, addr = acc_addr + buf * 256, next = acc_addr + (buf ^ 1u) * 256;
@@ -407,25 +409,25 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         const float s0 = a0 * w0;
         const uint64_t scale = pack2f(s0, s0);
         tc_wait_ld(v[0]);
-        tc_wait_ld(v[1]);
+        tmem_ld_32x32b_x32(addr + swap + 32, v[1]);
         fp8_pair_add(acc, 0, v[0], scale);
+        tc_wait_ld(v[1]);
         tmem_ld_32x32b_x32(addr + (64 - swap), v[0]);
         fp8_pair_add(acc, 16, v[1], scale);
-        tmem_ld_32x32b_x32(addr + (96 - swap), v[1]);
         tc_wait_ld(v[0]);
+        tmem_ld_32x32b_x32(addr + (96 - swap), v[1]);
+        fp8_pair_add(acc, 32, v[0], scale);
         tc_wait_ld(v[1]);
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(empty_bar + 8 * buf);
-        fp8_pair_add(acc, 32, v[0], scale);
+        fp8_pair_add(acc, 48, v[1], scale);
         if (more) {
           ok &= mbar_wait(&ctl->acc_full[buf ^ 1u], ((i + 1) >> 1) & 1u, abort_flag, st, 14);
           __syncwarp();
           tc_fence_after_sync();
           tmem_ld_32x32b_x32(next + swap, v[0]);
         }
-        fp8_pair_add(acc, 48, v[1], scale);
-        if (more) tmem_ld_32x32b_x32(next + swap + 32, v[1]);
         a0 = a1; w0 = w1; a1 = a2; w1 = w2;
       }
       const Fp8Tile done = tile;
