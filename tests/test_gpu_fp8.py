@@ -198,6 +198,17 @@ def test_tiles_of_cta_pairs(M, N, K, trans, out_dtype):
     assert torch.equal(c, ops.gemm_fp8(a, a_scale, w, trans_w=trans, out_dtype=out_dtype, token_tile=256))
 
 
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_rows_leave_before_an_empty_slab_takes_their_place(out_dtype):
+    """Contractions of one block: tiles follow so closely that a warp whose next 32 rows lie behind the last one comes
+    to its staging while the rows before are still on their way out."""
+    a, a_scale, w = operands(2476, 2936, 52, 3)
+    first = ops.gemm_fp8(a, a_scale, w, out_dtype=out_dtype, token_tile=256)
+    check_product(first, a, a_scale, w.codes, w.scales)
+    for _ in range(30):
+        assert torch.equal(first, ops.gemm_fp8(a, a_scale, w, out_dtype=out_dtype, token_tile=256))
+
+
 @pytest.mark.parametrize("token_tile", [16, 32, 128, 256])
 @pytest.mark.parametrize("trans", [False, True])
 def test_one_hot_rows_read_the_weight_back(token_tile, trans):

@@ -133,7 +133,7 @@ __device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, const CUt
 #pragma unroll
   for (int pass = 0; pass < 128 / kCols; ++pass) {
     const uint32_t box = stage + (pass & 1) * kPairBoxBytes;
-    if (lane == 0) tma_store_wait_read<1>();                  // the copy before last has read this box
+    if (lane == 0) tma_store_wait_read<1>();                  // the pass before last has left this box
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < 8; ++j) {                             // 16-byte chunks of this thread's row
@@ -154,10 +154,7 @@ __device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, const CUt
     if (whole) {
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        if (col < p.P) tma_store_2d_at(tmap_c, box, col, m_first);
-        tma_store_commit();
-      }
+      if (lane == 0 && col < p.P) tma_store_2d_at(tmap_c, box, col, m_first);
     } else {
       __syncwarp();
       const int chunk = lane & 7;
@@ -180,6 +177,8 @@ __device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, const CUt
       }
       __syncwarp();
     }
+    // a group for every pass, copied or not: the wait above counts passes
+    if (lane == 0) tma_store_commit();
   }
 }
 
