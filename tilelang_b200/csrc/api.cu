@@ -634,7 +634,7 @@ int run_gemm_fp8(const b200dq_fp8_gemm_args* a, const DeviceState* ds, cudaStrea
       const int size = out_elem_size(a->out_type);
       const cuuint64_t dims[2] = {static_cast<cuuint64_t>(outer), static_cast<cuuint64_t>(a->M)};
       const cuuint64_t strides[1] = {static_cast<cuuint64_t>(outer) * size};
-      const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / size), 32}, estr[2] = {1, 1};
+      const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / size), 128}, estr[2] = {1, 1};
       const CUtensorMapDataType type = a->out_type == OUT_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                        : a->out_type == OUT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
       const CUresult r = g_encode(&tmap_c, type, 2, a->c, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,

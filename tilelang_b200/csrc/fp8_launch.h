@@ -48,7 +48,7 @@ cudaError_t fp8_resident_clusters(int tile_tokens, int split, int* clusters);
 
 // CTA pairs, 256 tokens x 256 columns (p.p_tiles counts tiles of p.tile_cols); `pairs` clusters of two. With
 // gate_codes the columns of a tile are 128 of the gate's and 128 of the up half's, and c (bf16) may be null.
-// tmap_c: C with boxes of 32 rows x 128 bytes and the 128-byte swizzle, used where p.c_vec16 is set.
+// tmap_c: C with boxes of 128 rows x 128 bytes and the 128-byte swizzle, used where p.c_vec16 is set.
 cudaError_t launch_fp8_pair_gemm(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const CUtensorMap& tmap_c,
                                  const Fp8GemmParams& p, int pairs, cudaStream_t stream);
 constexpr int kFp8PairMaxGroups = 256;

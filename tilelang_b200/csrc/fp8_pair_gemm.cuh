@@ -18,8 +18,8 @@
 //
 // Persistent: one pair per two SMs, tiles in strips of 16 token tiles so that the tiles in flight
 // share their operands in L2. warp 0: TMA producer (both CTAs); warp 1: MMA issuer (first CTA);
-// warps 2, 3: tensor memory, tile table; warps 4-11: sums and output, which leaves through 8 KB of shared
-// memory per warp by TMA.
+// warp 2: tensor memory, output copies; warp 3: tile table; warps 4-11: sums and output, which leaves through
+// shared memory by TMA.
 //
 // GATED: weights are [gate; up], F rows each; the first CTA loads 128 gate rows, the second the 128 up
 // rows that belong to them, so that a tile's columns 0-127 and 128-255 are g and u of the same 128
@@ -36,8 +36,9 @@ constexpr int kPairThreads = 384;
 constexpr int kPairStages = 5;
 constexpr int kPairHalf = 128 * 128;                          // one operand's half tile: 128 rows x 128 bytes
 constexpr int kPairStageBytes = 2 * kPairHalf;
-constexpr int kPairBoxBytes = 32 * 128;                       // 32 output rows of 128 bytes: one store box
-constexpr int kPairStageOut = 2 * kPairBoxBytes;              // a warp's staging
+constexpr int kPairBoxBytes = 128 * 128;                      // 128 output rows of 128 bytes: one copy's box
+constexpr int kPairSlabBytes = 32 * 128;                      // a summing warp's rows of it
+constexpr int kPairOutBytes = 4 * kPairBoxBytes;              // two boxes for each half of the tile's columns
 constexpr int kPairStrip = 16;
 constexpr int kPairMaxGroups = 256;                           // groups whose tile table fits the control block
 // setmaxnreg moves registers from warps 0-3 to the eight summing warps: 128 * 40 + 256 * 232 = 384 * 168
@@ -46,12 +47,13 @@ constexpr int kPairOtherRegs = 40, kPairSumRegs = 232;
 struct Fp8PairCtl {
   uint64_t full[kPairStages], empty[kPairStages];
   uint64_t acc_full[2], acc_empty[2];
+  uint64_t out_full[2], out_empty[2];                         // boxes of a half of the columns: written, and copied
   uint32_t tmem_base;
   int abort_flag;
   int row_prefix[kPairMaxGroups + 1];
   int tile_prefix[kPairMaxGroups + 1];                        // token tiles before each group
 };
-constexpr int kPairSmemBytes = kPairStages * kPairStageBytes + 8 * kPairStageOut +
+constexpr int kPairSmemBytes = kPairStages * kPairStageBytes + kPairOutBytes +
                                static_cast<int>((sizeof(Fp8PairCtl) + 15) / 16 * 16);
 static_assert(kPairSmemBytes <= 232448, "shared memory of a CTA");
 
@@ -89,14 +91,27 @@ __device__ __forceinline__ void fp8_pair_prefixes(const Fp8GemmParams& p, Fp8Pai
   if (lane == 0) ctl->row_prefix[0] = ctl->tile_prefix[0] = 0;
 }
 
-// Where tile t lies: strips of kPairStrip token tiles, within a strip token tiles fastest. (The output has
-// 65536 elements a tile, so the tiles of any output that fits the GPU can be counted in 32 bits.)
+// n / d for n and d below 2^22 (inv = 1 / d): the rounded quotient is off by one at most. An integer division
+// takes some 200 cycles, three of them in a row between two tiles.
+__device__ __forceinline__ int div_small(int n, int d, float inv) {
+  int q = static_cast<int>(static_cast<float>(n) * inv);
+  const int r = n - q * d;
+  if (r < 0) --q;
+  if (r >= d) ++q;
+  return q;
+}
+
+// Where tile t lies: strips of kPairStrip token tiles, within a strip token tiles fastest. (An output of 2^22
+// tiles of 65536 elements would not fit the GPU.)
 __device__ __forceinline__ Fp8Tile fp8_pair_tile(const Fp8GemmParams& p, const Fp8PairCtl* ctl, int token_tiles, int t) {
-  const int strip = t / (kPairStrip * p.p_tiles);
-  const int in_strip = t - strip * (kPairStrip * p.p_tiles);
+  const int strip_tiles = kPairStrip * p.p_tiles;
+  const int strip = token_tiles <= kPairStrip ? 0 : div_small(t, strip_tiles, __fdividef(1.0f, static_cast<float>(strip_tiles)));
+  const int in_strip = t - strip * strip_tiles;
   const int high = min(kPairStrip, token_tiles - strip * kPairStrip);
-  const int tt = strip * kPairStrip + in_strip % high;
-  const int p0 = in_strip / high * p.tile_cols;
+  const int column = high == kPairStrip ? in_strip / kPairStrip
+                                        : div_small(in_strip, high, __fdividef(1.0f, static_cast<float>(high)));
+  const int tt = strip * kPairStrip + in_strip - column * high;
+  const int p0 = column * p.tile_cols;
   if (p.counts == nullptr) return Fp8Tile{0, tt * 256, p.M, p0};
   int lo = 0, hi = p.num_groups;                              // tile_prefix[lo] <= tt < tile_prefix[hi]
   while (hi - lo > 1) {
@@ -115,71 +130,107 @@ __device__ __forceinline__ uint4 ld_shared4(uint32_t addr) {
   return v;
 }
 
-// 32 rows x 128 columns of fp32 sums (thread = row) to C, 128 bytes of each row at a time through one of the
-// warp's two boxes in shared memory (16-byte chunks rotated by the row, as the tensor map's 128-byte
-// swizzle has them: no bank conflicts). Whole boxes leave by TMA, which reads them while the warp goes
-// on (moving the rows through registers again took three passes of the shared-memory pipe, 2450
-// cycles a tile); where a group ends inside the box, or C's rows do not start on 16 bytes, the warp writes.
-// `swap` = 64: the thread's first 64 columns are the tile's second 64 (gated u).
+// Whether this CTA's 128 rows leave by TMA, `rows` of them in C or in the group: a box may hang over the last row
+// of C, which the hardware cuts off, but not over the last row of a group.
+__device__ __forceinline__ bool pair_box_is_whole(const Fp8GemmParams& p, int rows) {
+  return p.c_vec16 && (rows >= 128 || (rows > 0 && p.counts == nullptr));
+}
+
+// A warp's 32 rows x 128 columns of fp32 sums (thread = row) to C, through its slab of the two boxes of its half
+// of the columns (128 bytes of each row, 16-byte chunks rotated by the row, as the tensor map's
+// 128-byte swizzle has them: no bank conflicts). Whole boxes leave by TMA, issued by a thread of another warp:
+// issuing keeps a thread for hundreds of cycles, which the next tile's sums would wait for. Where a group
+// ends inside the box, or C's rows do not start on 16 bytes, the warps write the rows. `rows`: of the CTA's
+// 128. `swap` = 64: the thread's first 64 columns are the tile's second 64 (gated u). `used`: rounds of the
+// boxes so far, counted by every summing warp and by the issuing one alike.
 template <int OUT_TYPE>
-__device__ __forceinline__ void fp8_pair_store(const Fp8GemmParams& p, const CUtensorMap* tmap_c, uint32_t stage,
-                                               const uint64_t (&acc)[64], int m_first, int rows, int col0, int swap,
-                                               int lane) {
+__device__ __forceinline__ bool fp8_pair_store(const Fp8GemmParams& p, Fp8PairCtl* ctl, int half, int quarter, uint32_t slab,
+                                               const uint64_t (&acc)[64], int m0, int rows, int col0, int swap, int lane,
+                                               uint32_t& used) {
   constexpr int kSize = OUT_TYPE == OUT_F32 ? 4 : 2;
-  constexpr int kCols = 128 / kSize;                          // columns of a pass
+  constexpr int kCols = 128 / kSize;                          // columns of a box
   const uint32_t out_rot = (lane & 7) << 4;
-  // a box may hang over the last row of C, which the hardware cuts off, but not over the last row of a group
-  const bool whole = p.c_vec16 && (rows == 32 || (rows > 0 && p.counts == nullptr));
+  const bool whole = pair_box_is_whole(p, rows);
+  bool ok = true;
 #pragma unroll
-  for (int pass = 0; pass < 128 / kCols; ++pass) {
-    const uint32_t box = stage + (pass & 1) * kPairBoxBytes;
-    if (lane == 0) tma_store_wait_read<1>();                  // the pass before last has left this box
+  for (int round = 0; round < 64 / kCols; ++round, ++used) {
+    ok &= mbar_wait(&ctl->out_empty[half], (used & 1u) ^ 1u, &ctl->abort_flag, p.status, 17);
     __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {                             // 16-byte chunks of this thread's row
+    for (int j = 0; j < 16; ++j) {                            // 16-byte chunks of this thread's row
       uint32_t h[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (OUT_TYPE == OUT_F32) {
-          const float2 f = unpack2(acc[pass * 16 + 2 * j + (i >> 1)]);
+          const float2 f = unpack2(acc[round * 32 + 2 * j + (i >> 1)]);
           h[i] = __float_as_uint(i & 1 ? f.y : f.x);
         } else {
-          const float2 f = unpack2(acc[pass * 32 + 4 * j + i]);
+          const float2 f = unpack2(acc[round * 64 + 4 * j + i]);
           h[i] = OUT_TYPE == OUT_BF16 ? bf162_as_u32(__floats2bfloat162_rn(f.x, f.y)) : h2_as_u32(__floats2half2_rn(f.x, f.y));
         }
       }
-      st_shared4(box + lane * 128 + ((j << 4) ^ out_rot), h);
+      st_shared4(slab + (j >> 3) * kPairBoxBytes + lane * 128 + (((j & 7) << 4) ^ out_rot), h);
     }
-    const int col = col0 + ((pass * kCols) ^ swap);
     if (whole) {
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0 && col < p.P) tma_store_2d_at(tmap_c, box, col, m_first);
     } else {
       __syncwarp();
       const int chunk = lane & 7;
-      const int c = col + chunk * (16 / kSize);
 #pragma unroll 1
-      for (int row = lane >> 3; row < rows; row += 4) {
-        const uint4 v = ld_shared4(box + row * 128 + ((chunk ^ (row & 7)) << 4));
-        uint8_t* dst = static_cast<uint8_t*>(p.c) + (static_cast<size_t>(m_first + row) * p.ldc + c) * kSize;
-        if (p.c_vec16 && c < p.P) {
-          *reinterpret_cast<uint4*>(dst) = v;
-        } else {
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      for (int k = 0; k < 2; ++k) {
+        const int c = col0 + (((round * 2 + k) * kCols) ^ swap) + chunk * (16 / kSize);
+#pragma unroll 1
+        for (int row = lane >> 3; row < 32 && quarter * 32 + row < rows; row += 4) {
+          const uint4 v = ld_shared4(slab + k * kPairBoxBytes + row * 128 + ((chunk ^ (row & 7)) << 4));
+          uint8_t* dst = static_cast<uint8_t*>(p.c) + (static_cast<size_t>(m0 + quarter * 32 + row) * p.ldc + c) * kSize;
+          if (p.c_vec16 && c < p.P) {
+            *reinterpret_cast<uint4*>(dst) = v;
+          } else {
+            const uint32_t e4[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-          for (int e = 0; e < 16 / kSize; ++e) {
-            if (c + e >= p.P) break;
-            if (kSize == 4) reinterpret_cast<uint32_t*>(dst)[e] = w[e];
-            else reinterpret_cast<uint16_t*>(dst)[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+            for (int e = 0; e < 16 / kSize; ++e) {
+              if (c + e >= p.P) break;
+              if (kSize == 4) reinterpret_cast<uint32_t*>(dst)[e] = e4[e];
+              else reinterpret_cast<uint16_t*>(dst)[e] = static_cast<uint16_t>(e4[e >> 1] >> (16 * (e & 1)));
+            }
           }
         }
       }
       __syncwarp();
     }
-    // a group for every pass, copied or not: the wait above counts passes
-    if (lane == 0) tma_store_commit();
+    if (lane == 0) mbar_arrive(&ctl->out_full[half]);
   }
+  return ok;
+}
+
+// The issuing thread's side of one tile: each half's boxes as its four warps have filled them.
+template <int OUT_TYPE, bool GATED>
+__device__ __forceinline__ bool fp8_pair_copy_out(const Fp8GemmParams& p, const CUtensorMap* tmap_c, Fp8PairCtl* ctl,
+                                                  uint32_t boxes, const Fp8Tile& tile, int rank, uint32_t& used) {
+  constexpr int kCols = OUT_TYPE == OUT_F32 ? 32 : 64;
+  const int m0 = tile.m0 + rank * 128;
+  const bool whole = pair_box_is_whole(p, tile.m_end - m0);
+#pragma unroll 1
+  for (int round = 0; round < 64 / kCols; ++round, ++used) {
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      if (!mbar_wait(&ctl->out_full[half], used & 1u, &ctl->abort_flag, p.status, 18)) return false;
+      if (!whole) continue;
+      const int swap = GATED && half == 1 ? 64 : 0;
+      const int col0 = tile.p0 + half * (GATED ? p.P / 2 : 128);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int col = col0 + (((round * 2 + k) * kCols) ^ swap);
+        if (col < p.P) tma_store_2d_at(tmap_c, boxes + (half * 2 + k) * kPairBoxBytes, col, m0);
+      }
+    }
+    tma_store_commit();
+    tma_store_wait_read<0>();
+    mbar_arrive(&ctl->out_empty[0]);
+    mbar_arrive(&ctl->out_empty[1]);
+  }
+  return true;
 }
 
 // acc[at ..] += scale * 32 columns, in pairs.
@@ -225,12 +276,10 @@ __device__ __forceinline__ float fp8_pair_act(uint64_t (&acc)[64], uint32_t part
 
 // The two warps of a lane quarter hold g and u of 32 tokens x 128 features, each its own 64 features in the
 // first half of `acc`. They swap the second halves, compute silu(g) u on 64 features each, agree
-// on the rows' maxima and write codes. `mine`, `partner`: the two warps' pairs of boxes.
+// on the rows' maxima and write codes. `mine`, `partner`: the two warps' slabs of their pairs of boxes.
 template <int FP8>
 __device__ __forceinline__ void fp8_pair_gate(const Fp8GemmParams& p, uint32_t mine, uint32_t partner, uint64_t (&acc)[64],
                                               int half, int quarter, int m_first, int rows, int f0, int lane) {
-  if (lane == 0) tma_store_wait_read<0>();                    // copies of h have read the boxes
-  __syncwarp();
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     const float2 a = unpack2(acc[32 + 2 * j]), b = unpack2(acc[32 + 2 * j + 1]);
@@ -278,7 +327,7 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   extern __shared__ __align__(1024) uint8_t fp8_pair_smem[];     // swizzle atoms start on 1 KiB boundaries
   uint8_t* smem = fp8_pair_smem;
   uint8_t* stage_out = smem + kPairStages * kPairStageBytes;
-  auto* ctl = reinterpret_cast<Fp8PairCtl*>(stage_out + 8 * kPairStageOut);
+  auto* ctl = reinterpret_cast<Fp8PairCtl*>(stage_out + kPairOutBytes);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int* abort_flag = &ctl->abort_flag;
   DeviceStatus* st = p.status;
@@ -287,6 +336,7 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   if (threadIdx.x == 0) {
     for (int i = 0; i < kPairStages; ++i) { mbar_init(&ctl->full[i], 1); mbar_init(&ctl->empty[i], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&ctl->acc_full[i], 1); mbar_init(&ctl->acc_empty[i], 16); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&ctl->out_full[i], 4); mbar_init(&ctl->out_empty[i], 1); }
     ctl->abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmap_a);
@@ -354,19 +404,31 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
           if (++s == kPairStages) { s = 0; phase ^= 1u; }
         }
       }
+    } else if (warp == 2 && lane == 0 && (!GATED || p.c != nullptr)) {
+      // ---------------- output copies of this CTA's rows ----------------
+      uint32_t used = 0;
+      bool ok = true;
+      for (int t = pair; ok && t < tiles; t += pairs) {
+        const Fp8Tile tile = fp8_pair_tile(p, ctl, token_tiles, t);
+        if (GATED || p.out_type != OUT_F32)
+          ok = fp8_pair_copy_out<OUT_BF16, GATED>(p, &tmap_c, ctl, smem_u32(stage_out), tile, rank, used);
+        else
+          ok = fp8_pair_copy_out<OUT_F32, GATED>(p, &tmap_c, ctl, smem_u32(stage_out), tile, rank, used);
+      }
+      tma_store_wait_read<0>();                               // copies have read their boxes before the memory goes away
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairSumRegs));
     // ---------------- sums: thread = one token of this CTA, 128 of the tile's columns ----------------
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t stage = smem_u32(stage_out + (warp - 4) * kPairStageOut);
-    const uint32_t other = smem_u32(stage_out + ((warp - 4) ^ 4) * kPairStageOut);
+    const uint32_t slab = smem_u32(stage_out + half * 2 * kPairBoxBytes + quarter * kPairSlabBytes);
+    const uint32_t other = smem_u32(stage_out + (half ^ 1) * 2 * kPairBoxBytes + quarter * kPairSlabBytes);
     const uint32_t empty_bar = cluster_map(smem_u32(&ctl->acc_empty[0]), 0);
     // gated, the warps of u take their columns in the order 64-127, 0-63: every warp then keeps its first 64
     const uint32_t swap = GATED && half == 1 ? 64 : 0;
     const uint32_t acc_addr = tmem_base + lane_addr + half * 128;
-    uint32_t i = 0;
+    uint32_t i = 0, used = 0;
     bool ok = true;
     // What a tile needs from memory: its scales, two blocks ahead (their latency is longer than a block's
     // multiplication). The next tile's first two are fetched before this one's rows are written.
@@ -431,25 +493,30 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       }
       const Fp8Tile done = tile;
       if (t + pairs < tiles) begin(t + pairs);
-      const int m_first = done.m0 + rank * 128 + quarter * 32;
+      const int m0 = done.m0 + rank * 128;
       ok = __all_sync(0xffffffffu, ok);                        // a wait that gave up: no lane writes
-      const int rows = ok ? min(32, done.m_end - m_first) : 0;
+      const int rows = ok ? done.m_end - m0 : 0;               // of this CTA's 128; may be none or more
       if (GATED) {
-        if (p.c != nullptr)
-          fp8_pair_store<OUT_BF16>(p, &tmap_c, stage, acc, m_first, rows, done.p0 + half * (p.P / 2), swap, lane);
+        if (p.c != nullptr) {
+          ok &= fp8_pair_store<OUT_BF16>(p, ctl, half, quarter, slab, acc, m0, rows, done.p0 + half * (p.P / 2), swap, lane, used);
+          // h has left both halves' boxes
+          ok &= mbar_wait(&ctl->out_empty[0], (used & 1u) ^ 1u, abort_flag, st, 17);
+          ok &= mbar_wait(&ctl->out_empty[1], (used & 1u) ^ 1u, abort_flag, st, 17);
+          __syncwarp();
+        }
         // both warps of a quarter meet in here, whatever happened to either
-        if (p.gate_fp8 == FP8_E4M3) fp8_pair_gate<FP8_E4M3>(p, stage, other, acc, half, quarter, m_first, rows, done.p0, lane);
-        else fp8_pair_gate<FP8_E5M2>(p, stage, other, acc, half, quarter, m_first, rows, done.p0, lane);
+        const int m_first = m0 + quarter * 32, mine = min(32, rows - quarter * 32);
+        if (p.gate_fp8 == FP8_E4M3) fp8_pair_gate<FP8_E4M3>(p, slab, other, acc, half, quarter, m_first, mine, done.p0, lane);
+        else fp8_pair_gate<FP8_E5M2>(p, slab, other, acc, half, quarter, m_first, mine, done.p0, lane);
       } else {
         const int col0 = done.p0 + half * 128;
-        if (p.out_type == OUT_BF16) fp8_pair_store<OUT_BF16>(p, &tmap_c, stage, acc, m_first, rows, col0, 0, lane);
-        else if (p.out_type == OUT_F16) fp8_pair_store<OUT_F16>(p, &tmap_c, stage, acc, m_first, rows, col0, 0, lane);
-        else fp8_pair_store<OUT_F32>(p, &tmap_c, stage, acc, m_first, rows, col0, 0, lane);
+        if (p.out_type == OUT_BF16) ok &= fp8_pair_store<OUT_BF16>(p, ctl, half, quarter, slab, acc, m0, rows, col0, 0, lane, used);
+        else if (p.out_type == OUT_F16) ok &= fp8_pair_store<OUT_F16>(p, ctl, half, quarter, slab, acc, m0, rows, col0, 0, lane, used);
+        else ok &= fp8_pair_store<OUT_F32>(p, ctl, half, quarter, slab, acc, m0, rows, col0, 0, lane, used);
       }
     }
   }
 
-  if (warp >= 4 && lane == 0) tma_store_wait_read<0>();       // copies have read their boxes before the memory goes away
   if (*abort_flag) {
     // copies in flight land before the shared memory goes away
     const uint64_t t0 = globaltimer_ns();
