@@ -6,7 +6,7 @@
 // one of two accumulators that fill tensor memory, and eight warps move them, scaled, to fp32
 // registers: thread = one token, 128 columns, one scale per block; 64 packed fmas.
 //
-// What bounds it (4096 x 28672 x 8192, 772 us in a burst, 2490 TFLOP/s, the GPU at its power limit near 1.5 GHz): the
+// What bounds it (4096 x 28672 x 8192, 760 us in a burst, 2530 TFLOP/s, the GPU at its power limit near 1.5 GHz): the
 // way round of an accumulator. Timestamps of one buffer, in cycles: hand-back seen to accumulator full 910
 // (four instructions of 128, issue, commit), first columns in registers 300, the rest read and added
 // 270, hand-back to the issuing warp 90; two buffers in turn make 780 a block, where the multiplication alone
