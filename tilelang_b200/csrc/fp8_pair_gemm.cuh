@@ -18,7 +18,7 @@
 //
 // Persistent: one pair per two SMs, tiles in strips of 16 token tiles so that the tiles in flight
 // share their operands in L2. warp 0: TMA producer (both CTAs); warp 1: MMA issuer (first CTA);
-// warp 2: tensor memory, output copies; warp 3: tile table; warps 4-11: sums and output, which leaves through
+// warp 2: tensor memory, output copies; warp 3: where tiles lie; warps 4-11: sums and output, which leaves through
 // shared memory by TMA.
 //
 // GATED: weights are [gate; up], F rows each; the first CTA loads 128 gate rows, the second the 128 up
@@ -48,6 +48,8 @@ struct Fp8PairCtl {
   uint64_t full[kPairStages], empty[kPairStages];
   uint64_t acc_full[2], acc_empty[2];
   uint64_t out_full[2], out_empty[2];                         // boxes of a half of the columns: written, and copied
+  uint64_t place_full[2], place_empty[2];                     // where the tile two, or one, ahead lies
+  Fp8Tile place[2];
   uint32_t tmem_base;
   int abort_flag;
   int row_prefix[kPairMaxGroups + 1];
@@ -337,6 +339,7 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     for (int i = 0; i < kPairStages; ++i) { mbar_init(&ctl->full[i], 1); mbar_init(&ctl->empty[i], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&ctl->acc_full[i], 1); mbar_init(&ctl->acc_empty[i], 16); }
     for (int i = 0; i < 2; ++i) { mbar_init(&ctl->out_full[i], 4); mbar_init(&ctl->out_empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&ctl->place_full[i], 1); mbar_init(&ctl->place_empty[i], 8); }
     ctl->abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmap_a);
@@ -416,6 +419,20 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
           ok = fp8_pair_copy_out<OUT_F32, GATED>(p, &tmap_c, ctl, smem_u32(stage_out), tile, rank, used);
       }
       tma_store_wait_read<0>();                               // copies have read their boxes before the memory goes away
+    } else if (warp == 3) {
+      // ---------------- the summing warps' tiles, ahead of them, and the first sectors of their scales into L1 ----------------
+      uint32_t n = 0;
+      for (int t = pair; t < tiles; t += pairs, ++n) {
+        if (!mbar_wait_warp(&ctl->place_empty[n & 1u], ((n >> 1) & 1u) ^ 1u, abort_flag, st, 19, lane)) break;
+        const Fp8Tile tile = fp8_pair_tile(p, ctl, token_tiles, t);
+        if (lane == 0) {
+          ctl->place[n & 1u] = tile;
+          mbar_arrive(&ctl->place_full[n & 1u]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          prefetch_l1(p.a_scale + static_cast<long long>(min(tile.m0 + rank * 128 + 32 * j + lane, p.M - 1)) * p.ld_a_scale);
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairSumRegs));
@@ -430,13 +447,17 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     const uint32_t acc_addr = tmem_base + lane_addr + half * 128;
     uint32_t i = 0, used = 0;
     bool ok = true;
-    // What a tile needs from memory: its scales, two blocks ahead (their latency is longer than a block's
-    // multiplication). The next tile's first two are fetched before this one's rows are written.
+    // Where a tile lies comes from warp 3 (divisions and, grouped, a search: some 400 cycles between two tiles). Its
+    // scales are fetched two blocks ahead (their latency is longer than a block's multiplication), the next
+    // tile's first two before this one's rows are written.
     Fp8Tile tile;
     const float *as = nullptr, *ws = nullptr;
     float a0 = 0.f, w0 = 0.f, a1 = 0.f, w1 = 0.f;
-    const auto begin = [&](int t) {
-      tile = fp8_pair_tile(p, ctl, token_tiles, t);
+    const auto begin = [&](uint32_t n) {
+      ok &= mbar_wait(&ctl->place_full[n & 1u], (n >> 1) & 1u, abort_flag, st, 20);
+      tile = ctl->place[n & 1u];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->place_empty[n & 1u]);
       // a tile may end before its second half; gated, the second half is the up half of the weight
       const int p_block = GATED ? (tile.p0 + half * (p.P / 2)) / 128 : min(tile.p0 / 128 + half, (p.P - 1) / 128);
       as = p.a_scale + static_cast<long long>(min(tile.m0 + rank * 128 + quarter * 32 + lane, p.M - 1)) * p.ld_a_scale;
@@ -445,7 +466,8 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       if (p.q_blocks > 1) { a1 = as[1]; w1 = ws[p.ws_q]; }
       as += 2; ws += 2 * p.ws_q;
     };
-    if (pair < tiles) begin(pair);
+    uint32_t n = 0;
+    if (pair < tiles) begin(0);
     for (int t = pair; t < tiles; t += pairs) {
       uint64_t acc[64];
 #pragma unroll
@@ -492,7 +514,7 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
         a0 = a1; w0 = w1; a1 = a2; w1 = w2;
       }
       const Fp8Tile done = tile;
-      if (t + pairs < tiles) begin(t + pairs);
+      if (t + pairs < tiles) begin(++n);
       const int m0 = done.m0 + rank * 128;
       ok = __all_sync(0xffffffffu, ok);                        // a wait that gave up: no lane writes
       const int rows = ok ? done.m_end - m0 : 0;               // of this CTA's 128; may be none or more

@@ -161,6 +161,8 @@ __device__ __forceinline__ void tma_store_2d_at(const CUtensorMap* tmap, uint32_
                : "memory");
 }
 
+__device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
+
 // ---- asynchronous 4-byte copies ----
 __device__ __forceinline__ void cp_async4(uint32_t smem_dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_dst), "l"(src) : "memory");
