@@ -503,7 +503,7 @@ struct Fp8Plan {
 //  - from 33 tokens on they own the lanes, half empty or not (measured in fp8_gemm.cuh);
 //  - from 129 tokens on CTA pairs with 256 x 256 tiles, unless there are so few of them that half the SMs
 //    would have none (256 tokens, 4096 x 4096: 14 us with 128-token tiles, 19 with pairs; at 14336
-//    rows of weight 36 and 21).
+//    rows of weight 34 and 21).
 Fp8Plan plan_fp8(int rows, int groups, int p_blocks, int sms, int token_tile) {
   Fp8Plan plan;
   const long long share = groups > 0 ? (rows + groups - 1) / groups : rows;

@@ -344,7 +344,8 @@ __global__ void __launch_bounds__(256) exchange_sum_kernel(const ExchangeSumPara
 // dy[row_of[t, s]] = w[t, s] dout[t] and dw[t, s] = <dout[t], y[row_of[t, s]]>: a warp takes a pair, the
 // warps of a CTA neighbouring pairs, so that a token's dout is read from memory once and from L1 after
 // that. No barrier: lanes' partial dot products are added by shuffles (a CTA per token, its
-// threads across the row and two barriers for every four slots, took 205 us where this takes 150).
+// threads across the row and two barriers for every four slots, took 205 us for 16384 x 6 rows of 2048, this
+// takes 133: the copy bandwidth).
 template <typename T>
 __global__ void __launch_bounds__(256) exchange_sum_grad_kernel(const ExchangeSumGradParams p) {
   chain_next();

@@ -6,7 +6,7 @@
 // scales differ from block to block, so every block of 128 gets an accumulator of its own in tensor
 // memory, and warps that read it back add it, scaled, to fp32 sums in registers. That costs one
 // fma per element and block on the fp32 pipe (128 lanes) against 128 multiply-adds on the tensor
-// pipe (8192 a cycle): half the tensor time, hidden behind it by two accumulators and packed fmas.
+// pipe (8192 a cycle): half the tensor time, hidden behind it by several accumulators and packed fmas.
 //
 // Weights are stored (P, Q), along the contraction, or for the gradient of the input (Q, P): the
 // same bytes, read through the other operand layout of the instruction, so no transposed copy.
@@ -98,8 +98,8 @@ __device__ __forceinline__ void fp8_store4(const Fp8GemmParams& p, long long m, 
 //     floats per block in shared memory, filled by 4-byte asynchronous copies.
 //   TOK_LANE = true, TN = 128: tokens own the lanes, 128 weight rows the columns; a reading thread then
 //     has one token and one scale per block (no vector of scales, half the fp32 work). Faster from 33
-//     tokens on, half empty as it is then (48 tokens, 14336 x 4096: 18 us against 22 in columns of 32 and 31
-//     in columns of 64, which need the vector of scales and more registers than two CTAs an SM leave).
+//     tokens on, half empty as it is then (48 tokens, 14336 x 4096: 17 us, in columns of 32 20; columns of 64
+//     measure the same 17 and would be one more kernel).
 // A cluster of up to 8 CTAs cuts the contraction, leaves its partial sums in shared memory, and every
 // CTA adds up a share of the tile from all of them in rank order: no scratch, one launch, and the
 // same bits every time.
