@@ -197,6 +197,46 @@ def test_other_layers_keep_their_results():
     assert torch.equal(moe.moe_forward(one, logits, k, E, mlp), moe.moe_forward(one.contiguous(), logits, k, E, mlp))
 
 
+def test_other_layers_with_a_router_wider_than_the_experts():
+    """Tokens whose experts all exist come out as ever; their neighbours' row indices stay inside the rows."""
+    E, k, T, H = 4, 2, 64, 128
+    x, logits = randn(T, H, seed=2, dtype=torch.bfloat16), randn(T, 2 * E, seed=3)
+    scale = torch.arange(1, E + 1, device=DEV, dtype=torch.bfloat16)
+    seen = []
+
+    def gemm(rows, counts):
+        which = torch.repeat_interleave(torch.arange(E, device=DEV), counts)
+        return rows * torch.cat((scale[which], scale.new_ones(rows.shape[0] - which.numel()))).unsqueeze(-1)
+
+    def combine(y, row_of, weights):
+        seen.append(((row_of >= 0) & (row_of < y.shape[0])).all())
+        return ops.moe_combine(y, row_of.clamp(0, y.shape[0] - 1), weights)
+
+    mlp = moe.ExpertMLP(gemm, lambda rows, counts: rows, lambda h: h, combine)
+    out = moe.moe_forward(x, logits, k, E, mlp)
+    assert len(seen) == 1 and seen[0]
+    weights, ids = moe.route(logits, k)
+    whole = (ids < E).all(1)
+    assert 0 < int(whole.sum()) < T
+    rows = x.unsqueeze(1) * scale[ids.clamp(max=E - 1)].unsqueeze(-1)            # rounded as the products round
+    want = (rows.double() * weights.double().unsqueeze(-1)).sum(1)
+    # one rounding of the sum, terms of one sign: 2^-8, and two fp32 ones
+    assert torch.allclose(out[whole].double(), want[whole], rtol=2 ** -8 + 2 ** -20, atol=0)
+
+
+def test_other_layers_can_be_differentiated_twice():
+    """An expert MLP of torch functions on the GPU: gradients of gradients, as before."""
+    E, k, T, H = 4, 2, 24, 16
+    x, logits = randn(T, H, seed=2).requires_grad_(), randn(T, E, seed=3)
+    mlp = moe.ExpertMLP(lambda rows, counts: rows ** 3, lambda rows, counts: rows, lambda h: h)
+    d_x, = torch.autograd.grad(moe.moe_forward(x, logits, k, E, mlp).sum(), x, create_graph=True)
+    dd_x, = torch.autograd.grad(d_x.sum(), x)
+    weights, _ = moe.route(logits, k)
+    want = 6 * x.detach().double() * weights.double().sum(1, keepdim=True)
+    # a handful of roundings of 2^-24 each
+    assert torch.allclose(dd_x.double(), want, rtol=2 ** -20, atol=0)
+
+
 def test_layer_in_graphs_and_on_another_stream():
     T, E, k, H, F = 300, 8, 3, 256, 128
     _, _, mlp = experts(E, H, F, 1)
