@@ -304,7 +304,7 @@ typedef struct b200dq_fp8_gemm_args {
 
 /* Sums are fp32: exact products added on the tensor cores within a block of 128, blocks scaled and
  * added in fp32 registers; one rounding to the output type. a, w, c and both pitches are multiples of
- * 16 bytes (c: of its element size). Deterministic; no scratch. Grouped: counts that do not sum to M
+ * 16 bytes (c: of its element size). Deterministic; no scratch. M, N, K up to 2^31 - 512. Grouped: counts that do not sum to M
  * are clamped to the rows that exist, and rows of C behind the last group are not written. */
 int b200dq_gemm_fp8(const b200dq_fp8_gemm_args* args, void* cuda_stream);
 
@@ -319,7 +319,7 @@ int b200dq_fp8_gated_fuses(int32_t M, int32_t N, int32_t K, int32_t num_groups);
  * x (tokens, width) go to out[row_of[t, s]]: copied, or with `scales` quantised as by
  * b200dq_quant_fp8 to fp8_type (out: rows of ld_out bytes). A pair whose id is outside
  * [0, num_experts) sorts behind the last expert: its row is zeros and row_of = -1 - row. scratch:
- * b200dq_exchange_scratch_bytes() bytes (may be 0). num_experts <= 1024. The reference's layer does
+ * b200dq_exchange_scratch_bytes() bytes (may be 0). num_experts <= 1024, width <= 2^28. The reference's layer does
  * this with argsort, bincount and gathers (examples/fusedmoe/example_fusedmoe_torch.py:65-91). */
 size_t b200dq_exchange_scratch_bytes(int64_t tokens, int32_t top_k, int32_t num_experts);
 int b200dq_exchange_dispatch(const void* experts, int32_t experts_int64, int64_t tokens, int32_t top_k,

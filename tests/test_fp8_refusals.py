@@ -126,3 +126,16 @@ def test_factory_checks():
                 dict(weight_dtype="bfloat16")):
         with pytest.raises(ValueError):
             tb.matmul_fp8_block(**{**dict(M=4, N=8, K=16), **bad})
+
+
+def test_sizes_whose_last_tile_would_pass_32_bits():
+    lib = _lib.load()
+    for change in (dict(M=2 ** 31 - 1), dict(N=2 ** 31 - 100, trans_w=1, lda=2 ** 31, ld_a_scale=2 ** 24), dict(M=2 ** 31 - 511),
+                   dict(K=2 ** 31 - 1, lda=2 ** 31, ldw=2 ** 31, ld_a_scale=2 ** 24)):
+        args = _lib.Fp8GemmArgs(**{**good(), **change})
+        assert lib.b200dq_gemm_fp8(ctypes.byref(args), None) == -1 and "2^31 - 512" in _lib.last_error(), change
+    wide = 2 ** 28 + 16                                              # rows of more than 2^30 bytes
+    for f, args in ((lib.b200dq_exchange_dispatch, [FAKE, 1, 1, 1, 4, FAKE, wide, wide, _lib.F32, FAKE, wide, None, 0, FAKE, FAKE, None, 0, None]),
+                    (lib.b200dq_exchange_sum, [FAKE, FAKE, None, FAKE, 1, 1, wide, _lib.F32, None]),
+                    (lib.b200dq_exchange_sum_grad, [FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1, 1, wide, _lib.F32, None])):
+        assert f(*args) == -1 and "2^28" in _lib.last_error()

@@ -553,6 +553,8 @@ int check_fp8_gemm(const b200dq_fp8_gemm_args* a) {
       (gated && a->gate_scales == nullptr))
     return fail("gemm_fp8: null pointer");
   if (a->M <= 0 || a->N <= 0 || a->K <= 0) return fail("gemm_fp8: M, N, K must be positive (got %d, %d, %d)", a->M, a->N, a->K);
+  // tiles that hang over an edge are still counted in 32 bits
+  if (std::max({a->M, a->N, a->K}) > 0x7fffffff - 511) return fail("gemm_fp8: M, N, K must not exceed 2^31 - 512 (got %d, %d, %d)", a->M, a->N, a->K);
   if (a->num_groups < 0 || a->num_groups > 65535) return fail("gemm_fp8: num_groups=%d outside [0, 65535]", a->num_groups);
   if (a->num_groups > 0 && a->counts == nullptr) return fail("gemm_fp8: a grouped call needs the counts");
   const int inner = a->trans_w ? a->N : a->K;
@@ -1048,6 +1050,7 @@ int b200dq_exchange_dispatch(const void* experts, int32_t experts_int64, int64_t
   if (tokens <= 0 || top_k <= 0 || width <= 0 || tokens > 0x7fffffffll / top_k)
     return fail("exchange_dispatch: tokens=%lld, top_k=%d, width=%d (tokens * top_k must stay below 2^31)", static_cast<long long>(tokens), top_k, width);
   if (num_experts <= 0 || num_experts > kExchangeMaxExperts) return fail("exchange_dispatch: num_experts=%d outside [1, %d]", num_experts, kExchangeMaxExperts);
+  if (width > kExchangeMaxWidth) return fail("exchange_dispatch: rows of %d columns, more than 2^28", width);
   if (type < EXCHANGE_F16 || type > EXCHANGE_F32) return fail("exchange_dispatch: rows must be f16, bf16 or f32");
   if (scales != nullptr && fp8_type != FP8_E4M3 && fp8_type != FP8_E5M2) return fail("exchange_dispatch: result must be e4m3 or e5m2");
   if (ld_x < width || ld_out < width) return fail("exchange_dispatch: a row pitch is less than the row");
@@ -1086,6 +1089,7 @@ int b200dq_exchange_sum(const void* y, const int64_t* row_of, const float* weigh
                         int32_t top_k, int32_t width, int32_t type, void* cuda_stream) {
   if (y == nullptr || row_of == nullptr || out == nullptr) return fail("exchange_sum: null pointer");
   if (tokens < 0 || top_k <= 0 || width <= 0) return fail("exchange_sum: tokens=%lld, top_k=%d, width=%d", static_cast<long long>(tokens), top_k, width);
+  if (width > kExchangeMaxWidth) return fail("exchange_sum: rows of %d columns, more than 2^28", width);
   if (type < EXCHANGE_F16 || type > EXCHANGE_F32) return fail("exchange_sum: rows must be f16, bf16 or f32");
   const int size = float_size(type);
   if (((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out)) & (size - 1)) != 0)
@@ -1110,6 +1114,7 @@ int b200dq_exchange_sum_grad(const void* d_out, const void* y, const int64_t* ro
   if (d_out == nullptr || row_of == nullptr || weights == nullptr || (d_weights != nullptr && y == nullptr))
     return fail("exchange_sum_grad: null pointer");
   if (tokens < 0 || top_k <= 0 || width <= 0) return fail("exchange_sum_grad: tokens=%lld, top_k=%d, width=%d", static_cast<long long>(tokens), top_k, width);
+  if (width > kExchangeMaxWidth) return fail("exchange_sum_grad: rows of %d columns, more than 2^28", width);
   if (type < EXCHANGE_F16 || type > EXCHANGE_F32) return fail("exchange_sum_grad: rows must be f16, bf16 or f32");
   const int size = float_size(type);
   if (((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(d_out) | reinterpret_cast<uintptr_t>(d_y)) & (size - 1)) != 0)

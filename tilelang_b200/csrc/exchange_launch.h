@@ -8,6 +8,7 @@ namespace b200dq {
 enum : int { EXCHANGE_F16 = 0, EXCHANGE_BF16 = 1, EXCHANGE_F32 = 2 };
 
 constexpr int kExchangeMaxExperts = 1024;
+constexpr int kExchangeMaxWidth = 1 << 28;       // bytes of a row are counted in 32 bits
 // Up to this many (token, slot) pairs every CTA counts all of them itself and sorting, copying and
 // quantising are one launch; above it two launches count and place, a third one moves the rows.
 constexpr int kExchangeOneLaunchPairs = 4096;
