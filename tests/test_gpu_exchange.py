@@ -178,6 +178,21 @@ def test_rows_outside_the_tensor_are_not_followed():
     assert (d_w[~kept] == 0).all() and (d_w[kept] != 0).all()
 
 
+def test_rows_that_no_index_names_have_no_gradient():
+    y, d = randn(12, 40, seed=1).requires_grad_(), randn(6, 40, seed=2)
+    row_of = torch.tensor([[0, 5], [12, 3], [2 ** 40, -1], [7, -2 ** 50], [1, 2], [-13, 4]], device=DEV)
+    w = torch.rand(6, 2, device=DEV, generator=gen(3))
+    want = torch.zeros_like(y.detach())
+    for t in range(6):
+        for s in range(2):
+            if 0 <= int(row_of[t, s]) < 12:
+                want[int(row_of[t, s])] = w[t, s] * d[t]
+    for _ in range(3):
+        torch.full((4096,), float("nan"), device=DEV)                # what an allocation may find
+        d_y, = torch.autograd.grad(moe.combine_rows(y, row_of, w), y, d)
+        assert torch.equal(d_y, want)
+
+
 def test_two_captured_graphs_share_nothing():
     experts = [pick(2000, 4, 16, 1), pick(2000, 4, 16, 2)]
     x = randn(2000, 64, seed=3, dtype=torch.bfloat16)

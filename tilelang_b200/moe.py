@@ -110,10 +110,12 @@ def make_gpu_expert_mlp(w1_packed, w2_packed, token_tile: Optional[int] = None) 
 class ExchangePlan:
     """Where every (token, slot) pair went: ``row_of`` (T, k) int64, the pair's row in expert order, or -1 - row
     for a pair whose expert id was outside [0, E) (its row lies behind the last expert's); ``counts`` (E,)
-    int64, the rows of each expert. Both stay on the device."""
+    int64, the rows of each expert. Both stay on the device. ``whole``: every row is some pair's, as it is in
+    the plans that :func:`dispatch` makes."""
 
     row_of: torch.Tensor
     counts: torch.Tensor
+    whole: bool = False
 
     @property
     def tokens(self) -> int:
@@ -151,7 +153,7 @@ def _exchange_out(x: torch.Tensor, experts: torch.Tensor, num_experts: int, out:
     lib = _lib.load()
     T, k = experts.shape
     plan = ExchangePlan(ops._new(T, k, torch.int64, x.device),
-                        torch.empty_strided((num_experts,), (1,), dtype=torch.int64, device=x.device))
+                        torch.empty_strided((num_experts,), (1,), dtype=torch.int64, device=x.device), True)
     if T == 0:
         plan.counts.zero_()
         return plan
@@ -197,8 +199,9 @@ def _exchange_sum(y: torch.Tensor, row_of: torch.Tensor, weights: Optional[torch
 
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, row_of, weights):
+    def forward(ctx, y, row_of, weights, whole):
         ctx.save_for_backward(y, row_of, weights)
+        ctx.whole = whole
         return _exchange_sum(y, row_of, weights)
 
     @staticmethod
@@ -207,13 +210,14 @@ class _Combine(torch.autograd.Function):
         y, row_of, weights = ctx.saved_tensors
         T, k = row_of.shape
         d_out = d_out.contiguous()
-        d_y = torch.empty_like(y) if ctx.needs_input_grad[0] else None
+        # the kernel writes the rows that the indices name: in a dispatch's plan that is all of them
+        d_y = (torch.empty_like if ctx.whole else torch.zeros_like)(y) if ctx.needs_input_grad[0] else None
         d_w = torch.empty_like(weights) if ctx.needs_input_grad[2] else None
         if T:
             ops._call(_lib.load().b200dq_exchange_sum_grad, "b200dq_exchange_sum_grad", y.device, d_out.data_ptr(),
                       y.data_ptr(), row_of.data_ptr(), weights.data_ptr(), d_y.data_ptr() if d_y is not None else None,
                       d_w.data_ptr() if d_w is not None else None, T, k, y.shape[1], ops._FLOAT_OF[y.dtype])
-        return d_y, None, d_w
+        return d_y, None, d_w, None
 
 
 def dispatch(x: torch.Tensor, experts: torch.Tensor, num_experts: int) -> Tuple[torch.Tensor, ExchangePlan]:
@@ -225,7 +229,7 @@ def dispatch(x: torch.Tensor, experts: torch.Tensor, num_experts: int) -> Tuple[
     experts = _check_experts(x, experts, num_experts)
     if torch.is_grad_enabled() and x.requires_grad:
         rows, row_of, counts = _Dispatch.apply(x, experts, num_experts)
-        return rows, ExchangePlan(row_of, counts)
+        return rows, ExchangePlan(row_of, counts, True)
     rows = ops._new(experts.numel(), x.shape[1], x.dtype, x.device)
     return rows, _exchange_out(x, experts, num_experts, rows, None, None)
 
@@ -244,7 +248,8 @@ def dispatch_fp8(x: torch.Tensor, experts: torch.Tensor, num_experts: int,
 
 
 def combine_rows(y: torch.Tensor, row_of: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
-    """:func:`combine` from the (T, k) row indices alone."""
+    """:func:`combine` from the (T, k) row indices alone. For a gradient of ``y`` no row may be named twice; rows
+    that no index names have the gradient zero."""
     return combine(y, ExchangePlan(row_of, row_of.new_empty(0)), weights)
 
 
@@ -267,7 +272,7 @@ def combine(y: torch.Tensor, plan: ExchangePlan, weights: torch.Tensor) -> torch
     weights = weights.float().contiguous()
     if not torch.is_grad_enabled() or not (y.requires_grad or weights.requires_grad):
         return _exchange_sum(y, row_of, weights)
-    return _Combine.apply(y, row_of, weights)
+    return _Combine.apply(y, row_of, weights, plan.whole)
 
 
 class _Fp8Mlp(torch.autograd.Function):
