@@ -210,7 +210,10 @@ class _Combine(torch.autograd.Function):
         y, row_of, weights = ctx.saved_tensors
         T, k = row_of.shape
         d_out = d_out.contiguous()
-        # the kernel writes the rows that the indices name: in a dispatch's plan that is all of them
+        # The kernel writes the rows that the indices name, zeros where -1 - row names one: in a dispatch's plan
+        # that is all of them. Elsewhere a negative index names none (-1 may stand for "no row").
+        if not ctx.whole:
+            row_of = row_of.masked_fill(row_of < 0, row_of.numel())
         d_y = (torch.empty_like if ctx.whole else torch.zeros_like)(y) if ctx.needs_input_grad[0] else None
         d_w = torch.empty_like(weights) if ctx.needs_input_grad[2] else None
         if T:
