@@ -139,3 +139,11 @@ def test_sizes_whose_last_tile_would_pass_32_bits():
                     (lib.b200dq_exchange_sum, [FAKE, FAKE, None, FAKE, 1, 1, wide, _lib.F32, None]),
                     (lib.b200dq_exchange_sum_grad, [FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1, 1, wide, _lib.F32, None])):
         assert f(*args) == -1 and "2^28" in _lib.last_error()
+
+
+def test_no_gradient_of_tokens_across_ranks():
+    w1 = ops.Fp8Weight(torch.zeros(2, 256, 128).to(torch.float8_e4m3fn), torch.ones(2, 2, 1))
+    w2 = ops.Fp8Weight(torch.zeros(2, 128, 128).to(torch.float8_e4m3fn), torch.ones(2, 1, 1))
+    x = torch.zeros(4, 128, dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(ValueError, match="no gradient of the tokens"):
+        moe.moe_forward_ep(x, torch.zeros(4, 2), 1, 2, moe.Fp8ExpertMLP(w1, w2))

@@ -311,7 +311,7 @@ class Fp8ExpertMLP(ExpertMLP):
     first product. Goes where :func:`make_gpu_expert_mlp`'s result goes (:func:`moe_forward`,
     :func:`moe_forward_ep`).
 
-    Differentiable in the tokens and the routing weights; the experts' weights are constants. The gradient is
+    Differentiable in the tokens (on one GPU) and the routing weights; the experts' weights are constants. The gradient is
     quantised like the activations, to ``grad_dtype``, and multiplied with the same weight bytes; the
     quantiser itself counts as the identity."""
 
@@ -381,7 +381,10 @@ def expert_ranges(num_experts: int, world_size: int) -> List[range]:
 def moe_forward_ep(x_local: torch.Tensor, logits_local: torch.Tensor, top_k: int, num_experts: int,
                    local_mlp: ExpertMLP, group: Optional[dist.ProcessGroup] = None) -> torch.Tensor:
     """Expert-parallel MoE layer. ``x_local`` are this rank's tokens; ``local_mlp`` runs this
-    rank's experts (counts are given for the local experts only, in order)."""
+    rank's experts (counts are given for the local experts only, in order). The exchange between the
+    ranks carries no gradient of the tokens."""
+    if isinstance(local_mlp, Fp8ExpertMLP) and torch.is_grad_enabled() and x_local.requires_grad:
+        raise ValueError("moe_forward_ep gives no gradient of the tokens (moe_forward does): call it under torch.no_grad(), or detach them")
     world = dist.get_world_size(group)
     rank = dist.get_rank(group)
     ranges = expert_ranges(num_experts, world)
