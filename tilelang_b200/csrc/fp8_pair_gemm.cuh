@@ -340,6 +340,7 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     for (int i = 0; i < 2; ++i) { mbar_init(&ctl->acc_full[i], 1); mbar_init(&ctl->acc_empty[i], 16); }
     for (int i = 0; i < 2; ++i) { mbar_init(&ctl->out_full[i], 4); mbar_init(&ctl->out_empty[i], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&ctl->place_full[i], 1); mbar_init(&ctl->place_empty[i], 8); }
+    ctl->place[0] = ctl->place[1] = Fp8Tile{0, 0, 0, 0};      // a valid place also after a wait that gave up
     ctl->abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmap_a);
