@@ -878,8 +878,8 @@ def run_moe(args, rank, world, local_rank):
         "grouped_gemms_only": {"ms": ms_gemm, "tflops": flops / ms_gemm / 1e9,
                                "frac_of_measured_bf16": flops / ms_gemm / 1e9 / world / peaks["bf16_tflops"],
                                "note": "W1 grouped GEMM + silu_mul + W2 grouped GEMM on evenly routed rows"},
-        # on one GPU the rows are sorted and moved by three launches more
-        "gpu_launches": (8 if world == 1 else 5) * args.steps * world, "clocks": clocks.summary(),
+        # two prefixes, two products, the activation and the weighted sum; on one GPU also count, place and move
+        "gpu_launches": (9 if world == 1 else 6) * args.steps * world, "clocks": clocks.summary(),
     }))
 
 
