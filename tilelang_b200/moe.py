@@ -358,12 +358,12 @@ def moe_forward(x: torch.Tensor, logits: torch.Tensor, top_k: int, num_experts: 
     weights, experts = route(logits, top_k)
     if isinstance(mlp, Fp8ExpertMLP):
         return mlp.layer(x, experts, weights, num_experts)
-    if (x.is_cuda and x.dtype in ops._FLOAT_OF and num_experts <= 1024 and x.dim() == 2 and x.shape[1] > 0
+    if (ops._ordinary(x, logits) and x.is_cuda and x.dtype in ops._FLOAT_OF and num_experts <= 1024 and x.dim() == 2 and x.shape[1] > 0
             and x.stride(1) == 1 and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1])
             and logits.shape[-1] <= num_experts and not (torch.is_grad_enabled() and x.requires_grad)):
         # the same order of rows as below, in one to three launches instead of some ten (a router wider than the
         # experts drops pairs, whose negative row indices `combine` need not know, and torch's gather can be
-        # differentiated more than once: both go on below)
+        # differentiated more than once, forwards, batched and recorded: all of these go on below)
         x_sorted, plan = dispatch(x, experts, num_experts)
         return mlp.combine(mlp(x_sorted, plan.counts), plan.row_of, weights.contiguous())
     order, token_of_row, counts = sort_by_expert(experts, num_experts)

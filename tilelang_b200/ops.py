@@ -13,6 +13,7 @@ from dataclasses import dataclass
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import (ACT_BF16, ACT_F16, ACT_I8, GF_FP4_SIMPLE, GF_HAS_BIAS, GF_ROW_SCALE, GF_TRANS_C, OUT_BF16, OUT_F16,
@@ -610,6 +611,19 @@ def _call(fn, what: str, device: torch.device, *args) -> None:
             rc = fn(*args, _raw_stream(idx))
     if rc:
         _lib.check(rc, what)
+
+
+def _ordinary(*tensors: torch.Tensor) -> bool:
+    """Whether the memory of these floating-point tensors is all there is to a call on them: no compilation or trace
+    that records torch's operators, no functorch transform, no dispatch mode, no tangent of forward-mode
+    differentiation, no subclass. A kernel reads the memory and passes by all of those."""
+    if torch.compiler.is_compiling() or torch._C._get_tracing_state() is not None:
+        return False
+    if torch._C._functorch.maybe_current_level() is not None or torch._C._len_torch_dispatch_stack() > 0:
+        return False
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        return False
+    return all(type(t) is torch.Tensor or type(t) is torch.nn.Parameter for t in tensors)
 
 
 def _blocks128(n: int) -> int:
