@@ -353,16 +353,25 @@ class Fp8ExpertMLP(ExpertMLP):
         return combine(self._run(codes, scales, plan.counts, x.dtype), plan, weights)
 
 
+def _fits_exchange(x: torch.Tensor, logits: torch.Tensor, top_k: int, num_experts: int) -> bool:
+    """Whether :func:`dispatch` takes these tokens and routes. A router wider than the experts drops pairs, whose negative
+    row indices an ``ExpertMLP.combine`` need not know; one of fewer rows than ``x`` leaves the other tokens out."""
+    return (x.dtype in ops._FLOAT_OF and x.dim() == 2 and 0 < x.shape[1] <= 1 << 28 and num_experts <= 1024
+            and x.stride(1) == 1 and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1])
+            and logits.dim() == 2 and logits.shape[0] == x.shape[0] and logits.shape[1] <= num_experts
+            and logits.shape[0] * top_k < 1 << 31)
+
+
 def moe_forward(x: torch.Tensor, logits: torch.Tensor, top_k: int, num_experts: int, mlp: ExpertMLP) -> torch.Tensor:
     """Single-device MoE layer: route, gather rows by expert, expert MLP, weighted combine."""
+    if logits.shape[0] > x.shape[0]:
+        raise ValueError(f"{logits.shape[0]} rows of logits for {x.shape[0]} tokens")
     weights, experts = route(logits, top_k)
     if isinstance(mlp, Fp8ExpertMLP):
         return mlp.layer(x, experts, weights, num_experts)
-    if (ops._ordinary(x, logits) and x.is_cuda and x.dtype in ops._FLOAT_OF and num_experts <= 1024 and x.dim() == 2 and x.shape[1] > 0
-            and x.stride(1) == 1 and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1])
-            and logits.shape[-1] <= num_experts and not (torch.is_grad_enabled() and x.requires_grad)):
-        # the same order of rows as below, in one to three launches instead of some ten (a router wider than the
-        # experts drops pairs, whose negative row indices `combine` need not know, and torch's gather can be
+    if (ops._ordinary(x, logits) and x.is_cuda and _fits_exchange(x, logits, top_k, num_experts)
+            and not (torch.is_grad_enabled() and x.requires_grad)):
+        # the same order of rows as below, in one to three launches instead of some ten (torch's gather can be
         # differentiated more than once, forwards, batched and recorded: all of these go on below)
         x_sorted, plan = dispatch(x, experts, num_experts)
         return mlp.combine(mlp(x_sorted, plan.counts), plan.row_of, weights.contiguous())
