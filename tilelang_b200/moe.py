@@ -169,6 +169,12 @@ def _exchange_out(x: torch.Tensor, experts: torch.Tensor, num_experts: int, out:
     return plan
 
 
+def _wants_gradient(*tensors: torch.Tensor) -> bool:
+    """Whether a call has to go through its autograd function: for a gradient, or because that refuses what it has no
+    rule for (a forward-mode tangent, a functorch transform), where the kernels would drop it."""
+    return (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) or ops._transformed(*tensors)
+
+
 class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, experts, num_experts):
@@ -230,7 +236,7 @@ def dispatch(x: torch.Tensor, experts: torch.Tensor, num_experts: int) -> Tuple[
     whose id lies outside [0, num_experts) -- a padded token's, say -- takes part in nothing: it gets a row of
     zeros behind the last expert's. Differentiable in x (float32 sums over the slots, in their order)."""
     experts = _check_experts(x, experts, num_experts)
-    if torch.is_grad_enabled() and x.requires_grad:
+    if _wants_gradient(x):
         rows, row_of, counts = _Dispatch.apply(x, experts, num_experts)
         return rows, ExchangePlan(row_of, counts, True)
     rows = ops._new(experts.numel(), x.shape[1], x.dtype, x.device)
@@ -273,7 +279,7 @@ def combine(y: torch.Tensor, plan: ExchangePlan, weights: torch.Tensor) -> torch
     if y.shape[0] != row_of.numel() or y.shape[1] == 0:
         raise ValueError(f"y must have {row_of.numel()} rows of at least one column, got {tuple(y.shape)}")
     weights = weights.float().contiguous()
-    if not torch.is_grad_enabled() or not (y.requires_grad or weights.requires_grad):
+    if not _wants_gradient(y, weights):
         return _exchange_sum(y, row_of, weights)
     return _Combine.apply(y, row_of, weights, plan.whole)
 
@@ -332,7 +338,7 @@ class Fp8ExpertMLP(ExpertMLP):
         """Rows sorted by expert -> rows. Rows behind the last expert's are undefined, their gradient is zero."""
         self._check(x_sorted)
         counts = ops._device_counts(counts, self.w1.num_groups, x_sorted.shape[0], x_sorted.device)
-        if torch.is_grad_enabled() and x_sorted.requires_grad:
+        if _wants_gradient(x_sorted):
             return _Fp8Mlp.apply(x_sorted, counts, self, True)
         return self._run(*ops.quant_fp8(x_sorted), counts, x_sorted.dtype)
 
@@ -345,7 +351,7 @@ class Fp8ExpertMLP(ExpertMLP):
         if num_experts != self.w1.num_groups:
             raise ValueError(f"the router has {num_experts} experts, the weights {self.w1.num_groups}")
         self._check(x)
-        if torch.is_grad_enabled() and x.requires_grad:
+        if _wants_gradient(x):
             rows, plan = dispatch(x, experts, num_experts)
             # the dispatch's gradient reads no row behind the last expert's
             return combine(_Fp8Mlp.apply(rows, plan.counts, self, False), plan, weights)
@@ -392,7 +398,7 @@ def moe_forward_ep(x_local: torch.Tensor, logits_local: torch.Tensor, top_k: int
     """Expert-parallel MoE layer. ``x_local`` are this rank's tokens; ``local_mlp`` runs this
     rank's experts (counts are given for the local experts only, in order). The exchange between the
     ranks carries no gradient of the tokens."""
-    if isinstance(local_mlp, Fp8ExpertMLP) and torch.is_grad_enabled() and x_local.requires_grad:
+    if isinstance(local_mlp, Fp8ExpertMLP) and _wants_gradient(x_local):
         raise ValueError("moe_forward_ep gives no gradient of the tokens (moe_forward does): call it under torch.no_grad(), or detach them")
     world = dist.get_world_size(group)
     rank = dist.get_rank(group)

@@ -613,15 +613,19 @@ def _call(fn, what: str, device: torch.device, *args) -> None:
         _lib.check(rc, what)
 
 
+def _transformed(*tensors: torch.Tensor) -> bool:
+    """Whether a functorch transform is at work, or one of these floating-point tensors carries a tangent."""
+    return torch._C._functorch.maybe_current_level() is not None or (
+        forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors))
+
+
 def _ordinary(*tensors: torch.Tensor) -> bool:
     """Whether the memory of these floating-point tensors is all there is to a call on them: no compilation or trace
     that records torch's operators, no functorch transform, no dispatch mode, no tangent of forward-mode
     differentiation, no subclass. A kernel reads the memory and passes by all of those."""
     if torch.compiler.is_compiling() or torch._C._get_tracing_state() is not None:
         return False
-    if torch._C._functorch.maybe_current_level() is not None or torch._C._len_torch_dispatch_stack() > 0:
-        return False
-    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    if torch._C._len_torch_dispatch_stack() > 0 or _transformed(*tensors):
         return False
     return all(type(t) is torch.Tensor or type(t) is torch.nn.Parameter for t in tensors)
 
