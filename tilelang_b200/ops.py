@@ -647,7 +647,7 @@ def _check_rows(name: str, t: torch.Tensor, device: Optional[torch.device] = Non
     rows, cols = t.shape
     if rows >= 1 << 31 or cols >= 1 << 31:
         raise ValueError(f"{name} has a side of 2^31 or more: {tuple(t.shape)}")
-    if cols > 1 and t.stride(1) != 1:
+    if rows > 0 and cols > 1 and t.stride(1) != 1:
         raise ValueError(f"{name} must have contiguous rows")
     if rows > 1 and t.stride(0) < cols:
         raise ValueError(f"{name} has rows that overlap")
@@ -798,7 +798,7 @@ def _fp8_gemm_args(what: str, a: torch.Tensor, a_scale: torch.Tensor, w: Fp8Weig
         raise ValueError("w.codes must have contiguous rows")
     ldw = stride[-2] if N > 1 else (K + 15) // 16 * 16
     group_stride = stride[0] if G > 1 else ldw * N
-    if M == 1:
+    if M <= 1:                                                       # no row follows another
         lda = (inner + 15) // 16 * 16
     a_ptr, w_ptr = a.data_ptr(), codes.data_ptr()
     if (a_ptr | lda | w_ptr | ldw | group_stride) % 16:
