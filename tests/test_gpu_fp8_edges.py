@@ -52,3 +52,21 @@ def test_layers_without_tokens(H, F):
         assert mlp(x, torch.zeros(3, dtype=torch.int64, device=DEV)).shape == (0, H)
         assert moe.moe_forward(x, torch.empty(0, 3, device=DEV), 2, 3, mlp).shape == (0, H)
     tb.check_status()
+
+
+def test_linear_of_one_strided_row():
+    """One token is taken in every layout that two are taken in."""
+    K, N = 200, 72
+    layer = tb.Fp8Linear.from_float(randn(N, K, seed=1))
+    base = randn(K, 5, seed=2, dtype=torch.bfloat16)
+    vector = randn(2 * K, seed=3, dtype=torch.bfloat16)
+    for x in (base.t()[:1], base.t()[2:3], base[:, 0], vector[::2], vector[::2].unsqueeze(0), base.t(), vector[:K].expand(3, K),
+              vector[:1].expand(K), vector[1:K + 1]):
+        want = layer(x.contiguous())
+        assert torch.equal(layer(x), want)
+        leaf = x.detach().requires_grad_()
+        d = randn(*want.shape[:-1], 2 * N, seed=4, dtype=torch.bfloat16)[..., ::2]
+        got, = torch.autograd.grad(layer(leaf), leaf, d)
+        other = x.detach().contiguous().requires_grad_()
+        assert torch.equal(got, torch.autograd.grad(layer(other), other, d.contiguous())[0])
+    assert torch.equal(tb.Fp8Linear.from_float(randn(N, 1, seed=5))(base[:, :1]), tb.Fp8Linear.from_float(randn(N, 1, seed=5))(base[:, :1].contiguous()))

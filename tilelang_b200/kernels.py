@@ -604,7 +604,7 @@ class Fp8Linear(torch.nn.Module):
         if x.shape[-1] != self.in_features:
             raise ValueError(f"Fp8Linear: expected {self.in_features} input features, got {x.shape[-1]}")
         x2 = x.reshape(-1, self.in_features)
-        if x2.shape[0] > 1 and (x2.stride(1) != 1 or x2.stride(0) < self.in_features):
+        if (x2.shape[1] > 1 and x2.stride(1) != 1) or (x2.shape[0] > 1 and x2.stride(0) < self.in_features):
             x2 = x2.contiguous()
         out = _Fp8Linear.apply(x2, self.weight.codes, self.weight.scales, self.grad_dtype)
         if self.bias is not None:
