@@ -291,11 +291,11 @@ typedef struct b200dq_fp8_gemm_args {
   int32_t a_type, w_type;   /* enum b200dq_fp8_type, any pairing                              */
   int32_t out_type;         /* f16, bf16 or f32                                               */
   int32_t trans_w;
-  int32_t token_tile;       /* 0: chosen; 16, 32: tokens are the tile's columns, 128: its lanes, 256: a CTA pair's */
+  int32_t token_tile;       /* 0: chosen; 16, 32: tokens are the tile's columns, 128: its lanes, 256: a CTA pair's (256 groups at most) */
   int32_t split;            /* 0: chosen; else CTAs (1 to 8) that share a tile's contraction  */
   /* Gated (NULL for none): N = 2F rows of W, gate above up, F a multiple of 128. Instead of h = A * W^T
    * the codes and scales of silu(h[:, :F]) * h[:, F:] are written, from the fp32 sums; c may be NULL,
-   * or takes h in bf16. */
+   * or takes h in bf16. Always on the 256-token tile, whose groups are at most 256. */
   void* gate_codes;         /* (M, F), rows of ld_gate bytes                                   */
   float* gate_scales;       /* (M, F / 128), contiguous                                        */
   int64_t ld_gate;

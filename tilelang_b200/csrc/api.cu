@@ -572,8 +572,9 @@ int check_fp8_gemm(const b200dq_fp8_gemm_args* a) {
     return fail("gemm_fp8: scales and output must be aligned to their elements");
   if (a->token_tile != 0 && a->token_tile != 16 && a->token_tile != 32 && a->token_tile != 128 && a->token_tile != 256)
     return fail("gemm_fp8: token_tile must be 0, 16, 32, 128 or 256 (got %d)", a->token_tile);
-  if (a->token_tile == 256 && a->num_groups > kFp8PairMaxGroups)
-    return fail("gemm_fp8: the 256-token tile takes at most %d groups", kFp8PairMaxGroups);
+  // a gated product takes the 256-token tile whatever token_tile says
+  if ((gated || a->token_tile == 256) && a->num_groups > kFp8PairMaxGroups)
+    return fail("gemm_fp8: the 256-token tile, and with it a gated product, takes at most %d groups (got %d)", kFp8PairMaxGroups, a->num_groups);
   if (a->token_tile == 256 && a->split > 1) return fail("gemm_fp8: the 256-token tile does not split the contraction");
   if (gated) {
     if (a->trans_w || a->N % 256 != 0) return fail("gemm_fp8: a gated product needs gate and up rows in multiples of 128 (N=%d) and no trans_w", a->N);
