@@ -26,3 +26,30 @@ def test_gated_products_of_more_groups_than_the_tile_table_holds(groups, more):
     assert lib.b200dq_gemm_fp8(ctypes.byref(args), None) == -1 and "at most 256 groups" in _lib.last_error()
     assert lib.b200dq_fp8_gated_fuses(1 << 20, 256, 256, groups) == 0
     assert lib.b200dq_fp8_gated_fuses(1 << 20, 256, 256, 256) == 1
+
+
+@pytest.mark.parametrize("change", [dict(a_scale=FAKE + 2), dict(w_scale=FAKE + 1), dict(c=FAKE + 1), dict(**{**GATED, "gate_scales": FAKE + 2}),
+                                    dict(num_groups=2, counts=FAKE + 2), dict(num_groups=2, counts=FAKE + 4, counts_int64=1),
+                                    dict(out_type=_lib.OUT_F32, c=FAKE + 2)])
+def test_products_refuse_pointers_between_elements(change):
+    args = product(**change)
+    assert _lib.load().b200dq_gemm_fp8(ctypes.byref(args), None) == -1 and "aligned" in _lib.last_error()
+
+
+def test_the_exchange_refuses_pointers_between_elements():
+    """Every array of a call: an address inside an element would be a misaligned access."""
+    lib = _lib.load()
+    # experts 0, int64 1, x 5, out 9, scales 11, row_of 13, counts 14, scratch 15
+    dispatch = [FAKE, 1, 8, 2, 4, FAKE, 64, 64, _lib.BF16, FAKE, 64, FAKE, 0, FAKE, FAKE, FAKE, 0, None]
+    total = [FAKE, FAKE, FAKE, FAKE, 8, 2, 64, _lib.F32, None]
+    grad = [FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 8, 2, 64, _lib.F32, None]
+    for f, args, wrong in ((lib.b200dq_exchange_dispatch, dispatch, [(0, 4), (5, 1), (11, 2), (13, 4), (14, 4), (15, 2)]),
+                           (lib.b200dq_exchange_sum, total, [(0, 2), (1, 4), (2, 2), (3, 2)]),
+                           (lib.b200dq_exchange_sum_grad, grad, [(0, 2), (1, 2), (2, 4), (3, 2), (4, 2), (5, 1)])):
+        for at, by in wrong:
+            bad = list(args)
+            bad[at] += by
+            assert f(*bad) == -1 and "aligned" in _lib.last_error(), (f.__name__, at)
+    ids32 = list(dispatch)
+    ids32[0], ids32[1] = FAKE + 2, 0
+    assert lib.b200dq_exchange_dispatch(*ids32) == -1 and "aligned" in _lib.last_error()

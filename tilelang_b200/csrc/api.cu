@@ -489,6 +489,9 @@ int run_gemm(const char* who, const b200dq_gemm_args* a, void* scratch, size_t s
   return fail("%s: no kernel for weight format %d with activation type %d", who, wf, act);
 }
 
+bool aligned_to(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+bool aligned16(const void* p) { return aligned_to(p, 16); }
+
 // ---- block-scaled fp8 products ---------------------------------------------------------------
 
 struct Fp8Plan {
@@ -565,11 +568,10 @@ int check_fp8_gemm(const b200dq_fp8_gemm_args* a) {
   if (a->ld_a_scale < (inner + 127) / 128) return fail("gemm_fp8: ld_a_scale=%lld is less than the %d scales of a row", static_cast<long long>(a->ld_a_scale), (inner + 127) / 128);
   if (a->a_type < 0 || a->a_type > FP8_E5M2 || a->w_type < 0 || a->w_type > FP8_E5M2) return fail("gemm_fp8: operands must be e4m3 or e5m2");
   if (a->out_type != OUT_F16 && a->out_type != OUT_BF16 && a->out_type != OUT_F32) return fail("gemm_fp8: output must be f16, bf16 or f32");
-  if ((reinterpret_cast<uintptr_t>(a->a) & 15) != 0 || (reinterpret_cast<uintptr_t>(a->w) & 15) != 0)
-    return fail("gemm_fp8: a and w must be 16-byte aligned");
-  if ((reinterpret_cast<uintptr_t>(a->a_scale) & 3) != 0 || (reinterpret_cast<uintptr_t>(a->w_scale) & 3) != 0 ||
-      (reinterpret_cast<uintptr_t>(a->c) & (out_elem_size(a->out_type) - 1)) != 0)
-    return fail("gemm_fp8: scales and output must be aligned to their elements");
+  if (!aligned16(a->a) || !aligned16(a->w)) return fail("gemm_fp8: a and w must be 16-byte aligned");
+  if (!aligned_to(a->a_scale, 4) || !aligned_to(a->w_scale, 4) || (gated && !aligned_to(a->gate_scales, 4)) ||
+      !aligned_to(a->c, out_elem_size(a->out_type)) || (a->num_groups > 0 && !aligned_to(a->counts, a->counts_int64 ? 8 : 4)))
+    return fail("gemm_fp8: scales, counts and output must be aligned to their elements");
   if (a->token_tile != 0 && a->token_tile != 16 && a->token_tile != 32 && a->token_tile != 128 && a->token_tile != 256)
     return fail("gemm_fp8: token_tile must be 0, 16, 32, 128 or 256 (got %d)", a->token_tile);
   // a gated product takes the 256-token tile whatever token_tile says
@@ -651,7 +653,6 @@ int run_gemm_fp8(const b200dq_fp8_gemm_args* a, const DeviceState* ds, cudaStrea
   return 0;
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 int float_size(int type) { return type == EXCHANGE_F32 ? 4 : 2; }
 
 }  // namespace
@@ -988,8 +989,7 @@ int b200dq_quant_fp8(int32_t mode, const void* x, int64_t ld_x, const void* d, i
   if (in_type < FP8_IN_F16 || in_type > FP8_IN_F32) return fail("quant_fp8: input must be f16, bf16 or f32");
   if (fp8_type != FP8_E4M3 && fp8_type != FP8_E5M2) return fail("quant_fp8: result must be e4m3 or e5m2");
   const int size = float_size(in_type);
-  if ((reinterpret_cast<uintptr_t>(x) & (size - 1)) != 0 || (reinterpret_cast<uintptr_t>(d) & (size - 1)) != 0 ||
-      (reinterpret_cast<uintptr_t>(scales) & 3) != 0)
+  if (!aligned_to(x, size) || !aligned_to(d, size) || !aligned_to(scales, 4))
     return fail("quant_fp8: pointers must be aligned to their elements");
   if (rows == 0) return 0;
   Fp8QuantParams p;
@@ -1017,7 +1017,7 @@ int b200dq_quant_fp8_blocks(const void* x, void* codes, int64_t ld_codes, float*
   if (ld_codes < K) return fail("quant_fp8_blocks: a row pitch is less than the row");
   if (in_type < FP8_IN_F16 || in_type > FP8_IN_F32) return fail("quant_fp8_blocks: input must be f16, bf16 or f32");
   if (fp8_type != FP8_E4M3 && fp8_type != FP8_E5M2) return fail("quant_fp8_blocks: result must be e4m3 or e5m2");
-  if ((reinterpret_cast<uintptr_t>(x) & (float_size(in_type) - 1)) != 0 || (reinterpret_cast<uintptr_t>(scales) & 3) != 0)
+  if (!aligned_to(x, float_size(in_type)) || !aligned_to(scales, 4))
     return fail("quant_fp8_blocks: pointers must be aligned to their elements");
   CUDA_OK(launch_fp8_quant_blocks(x, static_cast<uint8_t*>(codes), scales, batch, N, K, ld_codes, in_type, fp8_type,
                                   static_cast<cudaStream_t>(cuda_stream)));
@@ -1057,7 +1057,8 @@ int b200dq_exchange_dispatch(const void* experts, int32_t experts_int64, int64_t
   if (ld_x < width || ld_out < width) return fail("exchange_dispatch: a row pitch is less than the row");
   if (scales == nullptr && ld_out != width) return fail("exchange_dispatch: copied rows are contiguous");
   const int size = float_size(type);
-  if ((reinterpret_cast<uintptr_t>(x) & (size - 1)) != 0 || (scales == nullptr && (reinterpret_cast<uintptr_t>(out) & (size - 1)) != 0))
+  if (!aligned_to(x, size) || (scales == nullptr && !aligned_to(out, size)) || !aligned_to(scales, 4) ||
+      !aligned_to(experts, experts_int64 ? 8 : 4) || !aligned_to(row_of, 8) || !aligned_to(counts, 8) || !aligned_to(scratch, 4))
     return fail("exchange_dispatch: pointers must be aligned to their elements");
   if (scratch_bytes < b200dq_exchange_scratch_bytes(tokens, top_k, num_experts) ||
       (scratch == nullptr && b200dq_exchange_scratch_bytes(tokens, top_k, num_experts) > 0))
@@ -1093,7 +1094,7 @@ int b200dq_exchange_sum(const void* y, const int64_t* row_of, const float* weigh
   if (width > kExchangeMaxWidth) return fail("exchange_sum: rows of %d columns, more than 2^28", width);
   if (type < EXCHANGE_F16 || type > EXCHANGE_F32) return fail("exchange_sum: rows must be f16, bf16 or f32");
   const int size = float_size(type);
-  if (((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(out)) & (size - 1)) != 0)
+  if (!aligned_to(y, size) || !aligned_to(out, size) || !aligned_to(row_of, 8) || !aligned_to(weights, 4))
     return fail("exchange_sum: pointers must be aligned to their elements");
   if (tokens == 0) return 0;
   ExchangeSumParams p;
@@ -1118,7 +1119,8 @@ int b200dq_exchange_sum_grad(const void* d_out, const void* y, const int64_t* ro
   if (width > kExchangeMaxWidth) return fail("exchange_sum_grad: rows of %d columns, more than 2^28", width);
   if (type < EXCHANGE_F16 || type > EXCHANGE_F32) return fail("exchange_sum_grad: rows must be f16, bf16 or f32");
   const int size = float_size(type);
-  if (((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(d_out) | reinterpret_cast<uintptr_t>(d_y)) & (size - 1)) != 0)
+  if (!aligned_to(y, size) || !aligned_to(d_out, size) || !aligned_to(d_y, size) || !aligned_to(row_of, 8) ||
+      !aligned_to(weights, 4) || !aligned_to(d_weights, 4))
     return fail("exchange_sum_grad: pointers must be aligned to their elements");
   if (tokens == 0 || (d_y == nullptr && d_weights == nullptr)) return 0;
   ExchangeSumGradParams p;
