@@ -2,8 +2,10 @@
 import ctypes
 
 import pytest
+import torch
+from torch._subclasses import FakeTensorMode
 
-from tilelang_b200 import _lib
+from tilelang_b200 import _lib, moe, ops
 
 FAKE = 1 << 20                                  # an address that is never read: every call here is refused first
 
@@ -53,3 +55,29 @@ def test_the_exchange_refuses_pointers_between_elements():
     ids32 = list(dispatch)
     ids32[0], ids32[1] = FAKE + 2, 0
     assert lib.b200dq_exchange_dispatch(*ids32) == -1 and "aligned" in _lib.last_error()
+
+
+def test_sizes_that_the_c_calls_would_cut_to_32_bits():
+    """2^32 + 8 columns would arrive as 8 of them."""
+    with FakeTensorMode():                                           # sizes alone: nothing is allocated
+        def new(*shape, dtype=torch.bfloat16):
+            return torch.empty(*shape, dtype=dtype, device="cuda")
+
+        one = new(1, 1, dtype=torch.int64)
+        for width in (2 ** 28 + 8, 2 ** 32 + 8):
+            with pytest.raises(ValueError, match="2\\^28"):
+                moe.combine_rows(new(1, width), one, new(1, 1))
+        many = 2 ** 32 + 2
+        with pytest.raises(ValueError, match="2\\^31"):
+            moe.combine_rows(new(many, 8), new(1, many, dtype=torch.int64), new(1, many))
+        for dispatch in (moe.dispatch, moe.dispatch_fp8):
+            with pytest.raises(ValueError, match="2\\^31"):
+                dispatch(new(1, 8), new(1, many, dtype=torch.int64), 4)
+            with pytest.raises(ValueError, match="2\\^31"):
+                dispatch(new(2 ** 28, 8), new(2 ** 28, 8, dtype=torch.int64), 4)
+        for shape in ((1, 2 ** 32 + 8), (2 ** 32 + 8, 1), (1, 2 ** 31, 1)):
+            with pytest.raises(ValueError, match="2\\^31"):
+                ops.quant_fp8_weight(new(*shape))
+        for f in (ops.quant_fp8, ops.silu_mul_quant_fp8):
+            with pytest.raises(ValueError, match="2\\^31"):
+                f(new(1, 2 ** 32 + 256))

@@ -142,6 +142,8 @@ def _check_experts(x: torch.Tensor, experts: torch.Tensor, num_experts: int) -> 
         raise ValueError(f"experts is on {experts.device}, x on {x.device}")
     if experts.dim() != 2 or experts.shape[0] != x.shape[0] or experts.shape[1] == 0:
         raise ValueError(f"experts must have shape ({x.shape[0]}, top_k) with top_k at least 1, got {tuple(experts.shape)}")
+    if experts.numel() >= 1 << 31:
+        raise ValueError(f"experts must have fewer than 2^31 entries, got {tuple(experts.shape)}")
     if not 1 <= num_experts <= 1024:
         raise ValueError(f"num_experts must lie in 1 .. 1024, got {num_experts}")
     return experts.contiguous()
@@ -278,6 +280,8 @@ def combine(y: torch.Tensor, plan: ExchangePlan, weights: torch.Tensor) -> torch
         raise ValueError(f"weights must be floating point of shape {tuple(row_of.shape)}, got {weights.dtype} {tuple(weights.shape)}")
     if y.shape[0] != row_of.numel() or y.shape[1] == 0:
         raise ValueError(f"y must have {row_of.numel()} rows of at least one column, got {tuple(y.shape)}")
+    if y.shape[1] > 1 << 28 or row_of.shape[1] >= 1 << 31:           # the C call counts both in 32 bits
+        raise ValueError(f"rows have at most 2^28 columns and tokens fewer than 2^31 slots, got y {tuple(y.shape)} and row indices {tuple(row_of.shape)}")
     weights = weights.float().contiguous()
     if not _wants_gradient(y, weights):
         return _exchange_sum(y, row_of, weights)

@@ -757,8 +757,8 @@ def quant_fp8_weight(w: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) 
     _check_cuda_contig("w", w)
     if w.dim() not in (2, 3) or w.dtype not in _FLOAT_OF:
         raise ValueError("w must be a float16, bfloat16 or float32 tensor of two or three dimensions")
-    if w.numel() == 0:
-        raise ValueError("w must not be empty")
+    if w.numel() == 0 or max(w.shape) >= 1 << 31:
+        raise ValueError(f"w must not be empty, and its sides below 2^31, got {tuple(w.shape)}")
     lead, (N, K) = w.shape[:-2], w.shape[-2:]
     codes = torch.empty((*lead, N, (K + 15) // 16 * 16), dtype=dtype, device=w.device)[..., :K]
     scales = torch.empty((*lead, _blocks128(N), _blocks128(K)), dtype=torch.float32, device=w.device)
