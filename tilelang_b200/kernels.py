@@ -582,7 +582,10 @@ class Fp8Linear(torch.nn.Module):
     """A linear layer whose weight is kept in 8-bit floating point (:class:`ops.Fp8Weight`, (N, K)): the input is
     quantised per row and 128 columns, multiplied, and the bias (if any) added in the output dtype, which is the
     input's. Differentiable in the input (and bias); the weight is a constant. The incoming gradient is quantised
-    to ``grad_dtype`` and multiplied with the same weight bytes; the quantiser counts as the identity."""
+    to ``grad_dtype`` and multiplied with the same weight bytes; the quantiser counts as the identity.
+
+    The weight's ``codes`` and ``scales`` are buffers, and so is a bias that is no parameter: they are saved and moved with the module.
+    ``.half()`` and the like change the bias alone, since the weight's types are its format."""
 
     def __init__(self, weight: "ops.Fp8Weight", bias: Optional[torch.Tensor] = None,
                  grad_dtype: torch.dtype = torch.float8_e4m3fn):
@@ -590,8 +593,46 @@ class Fp8Linear(torch.nn.Module):
         ops._check_fp8_target(grad_dtype)
         if weight.codes.dim() != 2:
             raise ValueError("Fp8Linear: one (N, K) weight")
-        self.weight, self.bias, self.grad_dtype = weight, bias, grad_dtype
+        self.grad_dtype = grad_dtype
         self.in_features, self.out_features = weight.K, weight.N
+        self.register_buffer("codes", weight.codes)
+        self.register_buffer("scales", weight.scales)
+        if isinstance(bias, torch.nn.Parameter):
+            self.bias = bias
+        else:
+            self.register_buffer("bias", bias)
+
+    @property
+    def weight(self) -> "ops.Fp8Weight":
+        return ops.Fp8Weight(self.codes, self.scales)
+
+    @weight.setter
+    def weight(self, weight: "ops.Fp8Weight") -> None:
+        if weight.codes.shape != (self.out_features, self.in_features):
+            raise ValueError(f"Fp8Linear: expected codes of shape {(self.out_features, self.in_features)}, got {tuple(weight.codes.shape)}")
+        self.codes, self.scales = weight.codes, weight.scales
+
+    def _lay_out(self) -> None:
+        """Rows of the codes a multiple of 16 bytes apart, as the products read them: a copy to another device or
+        a loaded tensor packs them."""
+        if self.codes.shape[0] > 1 and self.codes.stride(0) % 16 != 0:
+            codes = ops._fp8_rows(*self.codes.shape, self.codes.dtype, self.codes.device)
+            self.codes = codes.copy_(self.codes)
+
+    def _apply(self, fn, recurse=True):
+        weight = (self.codes, self.scales)
+
+        def move(t):
+            new = fn(t)
+            return t.to(new.device) if new.dtype != t.dtype and (t is weight[0] or t is weight[1]) else new
+
+        super()._apply(move, recurse)
+        self._lay_out()
+        return self
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self._lay_out()
 
     @classmethod
     def from_float(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -606,7 +647,7 @@ class Fp8Linear(torch.nn.Module):
         x2 = x.reshape(-1, self.in_features)
         if (x2.shape[1] > 1 and x2.stride(1) != 1) or (x2.shape[0] > 1 and x2.stride(0) < self.in_features):
             x2 = x2.contiguous()
-        out = _Fp8Linear.apply(x2, self.weight.codes, self.weight.scales, self.grad_dtype)
+        out = _Fp8Linear.apply(x2, self.codes, self.scales, self.grad_dtype)
         if self.bias is not None:
             out = out + self.bias.to(out.dtype)
         return out.reshape(*x.shape[:-1], self.out_features)
