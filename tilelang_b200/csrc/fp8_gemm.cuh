@@ -217,7 +217,9 @@ fp8_tile_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
           umma_ss_f8(tmem_base + buf * TN, TOK_LANE ? t : w, TOK_LANE ? w : t, idesc, j != 0);
         }
         tc_commit(&ctl->acc_full[buf]);
-        tc_commit(&ctl->empty[s]);
+        // The last stages are not handed back: nobody would wait for them, and an arrival that nobody waits for may come
+        // when the CTA has left and its shared memory is someone else's.
+        if (kb + C::kStages < kb1) tc_commit(&ctl->empty[s]);
       }
       __syncwarp();
       if (++s == C::kStages) { s = 0; phase ^= 1u; }

@@ -388,6 +388,9 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       const uint32_t idesc = make_idesc_f8(p.a_fmt, p.w_fmt, 0, p.trans_w, 256, 256);
       const uint64_t w_step = p.trans_w ? 32 * 128 / 16 : 2;
       uint32_t s = 0, phase = 0, i = 0;
+      // Blocks of all of this pair's tiles. The last stages are not handed back: nobody would wait for them, and an
+      // arrival that nobody waits for may come when a CTA has left and its shared memory is someone else's.
+      const uint32_t blocks = pair < tiles ? static_cast<uint32_t>((tiles - pair - 1) / pairs + 1) * p.q_blocks : 0;
       bool ok = true;
       for (int t = pair; t < tiles; t += pairs) {
         for (int kb = 0; kb < p.q_blocks; ++kb, ++i) {
@@ -402,7 +405,7 @@ fp8_pair_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
             for (int j = 0; j < 4; ++j)
               umma_pair_ss_f8(acc, a_desc + 2 * j, w_desc + j * w_step, idesc, j != 0);
             tc_commit_pair(&ctl->acc_full[buf]);
-            tc_commit_pair(&ctl->empty[s]);
+            if (i + kPairStages < blocks) tc_commit_pair(&ctl->empty[s]);
           }
           __syncwarp();
           if (++s == kPairStages) { s = 0; phase ^= 1u; }
