@@ -174,7 +174,11 @@ def _exchange_out(x: torch.Tensor, experts: torch.Tensor, num_experts: int, out:
 def _wants_gradient(*tensors: torch.Tensor) -> bool:
     """Whether a call has to go through its autograd function: for a gradient, or because that refuses what it has no
     rule for (a forward-mode tangent, a functorch transform), where the kernels would drop it."""
-    return (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) or ops._transformed(*tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                return True
+    return ops._transformed(*tensors)
 
 
 class _Dispatch(torch.autograd.Function):

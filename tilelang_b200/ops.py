@@ -613,10 +613,14 @@ def _call(fn, what: str, device: torch.device, *args) -> None:
         _lib.check(rc, what)
 
 
+_functorch_level = torch._C._functorch.maybe_current_level
+
+
 def _transformed(*tensors: torch.Tensor) -> bool:
     """Whether a functorch transform is at work, or one of these floating-point tensors carries a tangent."""
-    return torch._C._functorch.maybe_current_level() is not None or (
-        forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors))
+    if _functorch_level() is not None:
+        return True
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _ordinary(*tensors: torch.Tensor) -> bool:
@@ -627,7 +631,10 @@ def _ordinary(*tensors: torch.Tensor) -> bool:
         return False
     if torch._C._len_torch_dispatch_stack() > 0 or _transformed(*tensors):
         return False
-    return all(type(t) is torch.Tensor or type(t) is torch.nn.Parameter for t in tensors)
+    for t in tensors:
+        if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
+            return False
+    return True
 
 
 def _blocks128(n: int) -> int:
