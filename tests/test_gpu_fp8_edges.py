@@ -70,3 +70,68 @@ def test_linear_of_one_strided_row():
         other = x.detach().contiguous().requires_grad_()
         assert torch.equal(got, torch.autograd.grad(layer(other), other, d.contiguous())[0])
     assert torch.equal(tb.Fp8Linear.from_float(randn(N, 1, seed=5))(base[:, :1]), tb.Fp8Linear.from_float(randn(N, 1, seed=5))(base[:, :1].contiguous()))
+
+
+# ---- many groups, skewed groups ------------------------------------------------------------------
+
+def check_grouped(out, a, a_scale, w, counts, trans):
+    """Rows against the definition in 64 bits. Bound: within a block of 128 at most 4 * 33 terms cut off at 2^-24 of the
+    largest, < 2^-16.9 of the sum of magnitudes; a rounding of 2^-24 per block and 11 more (scales, fma, join)."""
+    codes, scales = a.double(), a_scale.double()
+    av = codes * scales[:, torch.arange(a.shape[1], device=DEV) // 128]
+    blocks = -(-a.shape[1] // 128)
+    at = 0
+    for e, c in enumerate(counts):
+        if c == 0:
+            continue
+        wv = w.codes[e].double() * w.scales[e].double()[torch.arange(w.N, device=DEV) // 128][:, torch.arange(w.K, device=DEV) // 128]
+        wv = wv if trans else wv.t()
+        rows = av[at:at + c]
+        size = rows.abs() @ wv.abs()
+        assert ((out[at:at + c].double() - rows @ wv).abs() <= size * (2.0 ** -16.9 + (blocks + 11) * 2.0 ** -24)).all(), e
+        at += c
+    return at
+
+
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("counts,tile", [
+    ([140 + 7 * (i % 5) for i in range(300)], 0),        # more groups than CTA pairs take, a tile and more each
+    ([129] * 257, 0), ([200] * 256, 0),                  # either side of that limit
+    ([5000] + [1] * 511, 0), ([1] * 511 + [5000], 0),    # a mean share of 11 rows, and one group of 313 tiles of 16
+    ([0] * 400 + [3000] + [0] * 624, 16), ([700, 0, 1] * 100, 32),
+])
+def test_many_and_skewed_groups(counts, tile, trans):
+    N, K, G = 144, 272, len(counts)
+    rows = sum(counts) + 13
+    a, a_scale = ops.quant_fp8(randn(rows, N if trans else K, seed=G))
+    w = ops.quant_fp8_weight(randn(G, N, K, seed=G + 1, scale=0.05))
+    out = torch.full((rows, K if trans else N), 7.0, device=DEV)
+    ops.gemm_fp8_grouped(a, a_scale, w, torch.tensor(counts, device=DEV), trans_w=trans, out=out, token_tile=tile)
+    tb.check_status()
+    at = check_grouped(out, a, a_scale, w, counts, trans)
+    assert at == rows - 13 and (out[at:] == 7.0).all()
+
+
+@pytest.mark.parametrize("G,each", [(256, 200), (257, 200), (300, 140)])
+def test_gated_products_either_side_of_256_groups(G, each):
+    """Fused up to 256 groups, a product in float32 and a quantiser above. The codes stand for the activation to half a
+    step (2^-4, 2^-10 of the scale for the smallest) and what the product's bound, 2^-16.5 of the sum of magnitudes, moves
+    it by (|silu'| <= 1.1)."""
+    F, K = 128, 256
+    a, a_scale = ops.quant_fp8(randn(G * each, K, seed=1))
+    w = ops.quant_fp8_weight(randn(G, 2 * F, K, seed=2, scale=0.05))
+    counts = torch.full((G,), each, device=DEV)
+    codes, scales = ops.gemm_fp8_gated(a, a_scale, w, counts)
+    tb.check_status()
+    if G > 256:
+        want = ops.silu_mul_quant_fp8(ops.gemm_fp8_grouped(a, a_scale, w, counts, out_dtype=torch.float32))
+        assert torch.equal(codes.float(), want[0].float()) and torch.equal(scales, want[1])
+    av = (a.double() * a_scale.double()[:, torch.arange(K, device=DEV) // 128]).view(G, each, K)
+    wv = w.codes.double() * w.scales.double()[:, torch.arange(2 * F, device=DEV) // 128][:, :, torch.arange(K, device=DEV) // 128]
+    ref, size = torch.bmm(av, wv.transpose(1, 2)).flatten(0, 1), torch.bmm(av.abs(), wv.abs().transpose(1, 2)).flatten(0, 1) * 2.0 ** -16.5
+    (g, u), (dg, du) = ref.split(F, -1), size.split(F, -1)
+    v = torch.sigmoid(g) * g * u
+    slack = 1.1 * dg * u.abs() + g.abs() * du + 2.0 ** -20 * v.abs()
+    s = scales.double()
+    off = (codes.double() * s - v).abs()
+    assert (off <= (v.abs() + slack) * 2.0 ** -4 + s * 2.0 ** -10 * 1.001 + slack).all()
