@@ -93,18 +93,18 @@ __device__ __forceinline__ void fp8_pair_prefixes(const Fp8GemmParams& p, Fp8Pai
   if (lane == 0) ctl->row_prefix[0] = ctl->tile_prefix[0] = 0;
 }
 
-// n / d for n and d below 2^22 (inv = 1 / d): the rounded quotient is off by one at most. An integer division
-// takes some 200 cycles, three of them in a row between two tiles.
+// n / d (inv = 1 / d to 2 units in the last place): the rounded quotient is off by one at most below 2^21, and by three
+// for the most column tiles that an output can have, 2^23; the remainder, exact in 32 bits, puts it right. An
+// integer division takes some 200 cycles, three of them in a row between two tiles.
 __device__ __forceinline__ int div_small(int n, int d, float inv) {
   int q = static_cast<int>(static_cast<float>(n) * inv);
-  const int r = n - q * d;
-  if (r < 0) --q;
-  if (r >= d) ++q;
+  int r = static_cast<int>(static_cast<unsigned>(n) - static_cast<unsigned>(q) * static_cast<unsigned>(d));
+  for (; r < 0; r += d) --q;
+  for (; r >= d; r -= d) ++q;
   return q;
 }
 
-// Where tile t lies: strips of kPairStrip token tiles, within a strip token tiles fastest. (An output of 2^22
-// tiles of 65536 elements would not fit the GPU.)
+// Where tile t lies: strips of kPairStrip token tiles, within a strip token tiles fastest.
 __device__ __forceinline__ Fp8Tile fp8_pair_tile(const Fp8GemmParams& p, const Fp8PairCtl* ctl, int token_tiles, int t) {
   const int strip_tiles = kPairStrip * p.p_tiles;
   const int strip = token_tiles <= kPairStrip ? 0 : div_small(t, strip_tiles, __fdividef(1.0f, static_cast<float>(strip_tiles)));
