@@ -135,3 +135,28 @@ def test_gated_products_either_side_of_256_groups(G, each):
     s = scales.double()
     off = (codes.double() * s - v).abs()
     assert (off <= (v.abs() + slack) * 2.0 ** -4 + s * 2.0 ** -10 * 1.001 + slack).all()
+
+
+@pytest.mark.parametrize("dtype,rows", [(torch.float8_e4m3fn, 2000), (torch.float8_e5m2, 2000), (torch.float8_e4m3fn, 40)])
+def test_gated_codes_are_the_nearest_but_at_borders(dtype, rows):
+    """Fused and not: a code other than that of the 64-bit quotient is its neighbour, and the border between the two is
+    no further from the quotient than the product's bound (2^-16.5 of the sum of magnitudes) and 2^-20 of the value allow."""
+    F, K = 256, 512
+    a, a_scale = ops.quant_fp8(randn(rows, K, seed=1))
+    w = ops.quant_fp8_weight(randn(2 * F, K, seed=2, scale=0.05))
+    codes, scales = ops.gemm_fp8_gated(a, a_scale, w, dtype=dtype)
+    av = a.double() * a_scale.double()[:, torch.arange(K, device=DEV) // 128]
+    wv = w.codes.double() * w.scales.double()[torch.arange(2 * F, device=DEV) // 128][:, torch.arange(K, device=DEV) // 128]
+    (g, u), (dg, du) = (av @ wv.t()).split(F, -1), ((av.abs() @ wv.abs().t()) * 2.0 ** -16.5).split(F, -1)
+    s = scales.double()[:, torch.arange(F, device=DEV) // 128]
+    v = torch.sigmoid(g) * g * u
+    q, slack = v / s, (1.1 * dg * u.abs() + g.abs() * du + 2.0 ** -20 * v.abs()) / s
+    nearest, got = q.to(dtype).double(), codes.double()
+    other = got != nearest
+    assert other.double().mean() <= 1e-3
+    assert ((q - (got + nearest) / 2).abs() <= slack)[other].all()
+    step = torch.maximum(nearest.abs(), got.abs()) * (2.0 ** -3 if dtype == torch.float8_e4m3fn else 2.0 ** -2) + 2.0 ** (-9 if dtype == torch.float8_e4m3fn else -16)
+    assert ((got - nearest).abs() <= step).all()
+    for _ in range(3):
+        again = ops.gemm_fp8_gated(a, a_scale, w, dtype=dtype)
+        assert torch.equal(again[0].float(), codes.float()) and torch.equal(again[1], scales)
