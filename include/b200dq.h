@@ -302,8 +302,8 @@ typedef struct b200dq_fp8_gemm_args {
   int32_t gate_type;        /* enum b200dq_fp8_type                                            */
 } b200dq_fp8_gemm_args;
 
-/* Sums are fp32: exact products added on the tensor cores within a block of 128, blocks scaled and
- * added in fp32 registers; one rounding to the output type. a, w, c and both pitches are multiples of
+/* Sums are fp32: exact products added on the tensor cores within a block of 128, blocks scaled (by the
+ * product of their two scales, which has to be in fp32's range) and added in fp32 registers; one rounding to the output type. a, w, c and both pitches are multiples of
  * 16 bytes (c: of its element size). Deterministic; no scratch. M, N, K up to 2^31 - 512. Grouped: counts that do not sum to M
  * are clamped to the rows that exist, and rows of C behind the last group are not written. */
 int b200dq_gemm_fp8(const b200dq_fp8_gemm_args* args, void* cuda_stream);

@@ -1,7 +1,7 @@
 // The product of fp8_gemm.cuh for many tokens: CTA pairs, tiles of 256 tokens x 256 weight rows.
 //
 // A pair of CTAs on two SMs works on one tile with tcgen05.mma.cta_group::2 (M = N = 256): each CTA
-// loads 128 tokens and 128 weight rows per block of 128, 32 KB for 8.4 million multiply-adds, two thirds
+// loads 128 tokens and 128 weight rows per block of 128, 32 KB for its 4.2 million multiply-adds, two thirds
 // of what a 128 x 256 tile of its own would pull through L2 for the same work. Its 128 x 256 sums per block go to
 // one of two accumulators that fill tensor memory, and eight warps move them, scaled, to fp32
 // registers: thread = one token, 128 columns, one scale per block; 64 packed fmas.

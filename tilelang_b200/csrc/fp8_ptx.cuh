@@ -149,7 +149,7 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
 }
 // Arrival on a barrier of the other CTA (or this one): says that tensor memory has been read, which the
 // tcgen05 fence in front of it orders; no ordinary memory is handed over, so it needs no cluster-wide
-// release (that form costs a memory barrier of about a microsecond: 1916 against 940 us at 4096 x 28672 x 8192).
+// release (with .release.cluster 4096 x 28672 x 8192 took 1916 us, without it 940).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }

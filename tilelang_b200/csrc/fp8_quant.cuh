@@ -58,7 +58,7 @@ __device__ __forceinline__ uint32_t fp8_pair(float lo, float hi) {
 
 // 1 / (1 + e^-g) from the hardware's base-2 exponential and reciprocal, a relative error of at most
 // |g| 2^-24 + 2^-21 (the rounded exponent, then 2 and 1 units in the last place): far below the codes' half
-// step. For g so low that e^-g overflows the result is 0. (The library's expf and an IEEE division made
+// step. Below g = -87.3, where it would be less than 2^-126, the result is 0. (The library's expf and an IEEE division made
 // the gradient's quantiser bound by instructions: 72 us for 24576 x 1408, of which the bytes need 42.)
 __device__ __forceinline__ float sigmoid_of(float g) {
   float e, r;

@@ -6,11 +6,10 @@ examples/fusedmoe/example_fusedmoe_torch.py (routing :26-40: softmax then
 argsort/bincount and score-weighted combine :65-91) and from its grouped GEMM
 (examples/grouped_gemm/example_grouped_gemm_fwd.py:8-36: rows sorted by expert, one
 weight per expert). Here the two grouped GEMMs and the activation between them are this
-library's kernels; routing, the row gather and the weighted scatter-add are torch
-tensor plumbing around them.
-
-On a GPU the rows are sorted and moved by this library too (:func:`dispatch`, :func:`combine`, both
-differentiable), and :class:`Fp8ExpertMLP` runs the experts in 8-bit floating point.
+library's kernels, and on a GPU so is what sorts, moves and adds up the rows (:func:`dispatch`,
+:func:`combine`, both differentiable in reverse mode); routing is torch's. Torch's sort and gather take
+over where more than the values is asked of a layer over torch functions (gradients of the tokens,
+forward mode, vmap, traces) and across ranks. :class:`Fp8ExpertMLP` runs the experts in 8-bit floating point.
 
 Expert parallelism: experts are split contiguously over the ranks, tokens start out
 partitioned by rank; one all-to-all sends every (token, expert) row to the rank that
@@ -240,7 +239,7 @@ def dispatch(x: torch.Tensor, experts: torch.Tensor, num_experts: int) -> Tuple[
     (T * k, H) in x's dtype. ``x`` (T, H) float16, bfloat16 or float32, its rows any distance apart;
     ``experts`` (T, k) int32 or int64. Rows of one expert keep the order of their (token, slot) pairs. A pair
     whose id lies outside [0, num_experts) -- a padded token's, say -- takes part in nothing: it gets a row of
-    zeros behind the last expert's. Differentiable in x (float32 sums over the slots, in their order)."""
+    zeros behind the last expert's. Differentiable in x (reverse mode; float32 sums over the slots, in their order)."""
     experts = _check_experts(x, experts, num_experts)
     if _wants_gradient(x):
         rows, row_of, counts = _Dispatch.apply(x, experts, num_experts)
@@ -271,7 +270,7 @@ def combine_rows(y: torch.Tensor, row_of: torch.Tensor, weights: torch.Tensor) -
 def combine(y: torch.Tensor, plan: ExchangePlan, weights: torch.Tensor) -> torch.Tensor:
     """Back from expert order: ``out[t] = sum_s weights[t, s] * y[plan.row_of[t, s]]``, float32 sums in slot order
     rounded once to y's dtype; dropped pairs add nothing. ``y`` (T * k, H) contiguous float16, bfloat16 or float32,
-    ``weights`` (T, k) of any floating type. Differentiable in y and weights."""
+    ``weights`` (T, k) of any floating type. Differentiable in y and weights (reverse mode)."""
     ops._check_cuda_contig("y", y)
     if y.dim() != 2 or y.dtype not in ops._FLOAT_OF:
         raise ValueError("y must be a 2-D float16, bfloat16 or float32 tensor")
@@ -325,7 +324,8 @@ class Fp8ExpertMLP(ExpertMLP):
     first product. Goes where :func:`make_gpu_expert_mlp`'s result goes (:func:`moe_forward`,
     :func:`moe_forward_ep`).
 
-    Differentiable in the tokens (on one GPU) and the routing weights; the experts' weights are constants. The gradient is
+    Tokens are float16 or bfloat16: the backward pass keeps h, and the gradient that meets it, in bfloat16. Differentiable
+    in the tokens (on one GPU) and the routing weights, in reverse mode; the experts' weights are constants. The gradient is
     quantised like the activations, to ``grad_dtype``, and multiplied with the same weight bytes; the
     quantiser itself counts as the identity."""
 

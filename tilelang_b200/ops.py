@@ -709,7 +709,8 @@ def quant_fp8(x: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn):
     ``scale = max|x| / 448`` (57344 for e5m2), at least 2^-126; ``code = rn(x / scale)``, ties to even, with the
     quotient taken as ``x * (1 / scale)`` in float32. A block that holds NaN or an infinity gets that as
     its scale, so that it does not come out of a product as a finite number. Rows of ``x`` may lie any distance apart;
-    the codes' rows lie a multiple of 16 bytes apart, as :func:`gemm_fp8` reads them."""
+    the codes' rows lie a multiple of 16 bytes apart, as :func:`gemm_fp8` reads them. Neither this nor the products
+    record a gradient: :class:`kernels.Fp8Linear` and :class:`moe.Fp8ExpertMLP` do."""
     return _quant_fp8(_lib.FP8_OF_ROWS, "quant_fp8", x, None, dtype)
 
 
@@ -849,7 +850,8 @@ def gemm_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: Fp8Weight, trans_w: bool
     """``C = A @ W^T`` with ``a`` (M, K) codes and ``a_scale`` (M, ceil(K / 128)) from :func:`quant_fp8`, ``w`` an
     (N, K) :class:`Fp8Weight`; C is (M, N) in float16, bfloat16 or float32. With ``trans_w`` it is
     ``C = A @ W`` with ``a`` (M, N): the gradient of the input, (M, K), from the same weight.
-    The two operands may be of different 8-bit types. Sums are float32 throughout, the result is rounded once.
+    The two operands may be of different 8-bit types. Sums are float32 throughout, the result is rounded once. The two
+    scales of a block are multiplied with one another first: their product has to be in float32's range.
     ``token_tile`` (16, 32, 128 or 256) and ``split`` (1 to 8) override the kernel's tile and the CTAs that
     share its contraction; 0 leaves them to the library."""
     args = _fp8_gemm_args("gemm_fp8", a, a_scale, w, trans_w, grouped=False)
