@@ -160,3 +160,22 @@ def test_gated_codes_are_the_nearest_but_at_borders(dtype, rows):
     for _ in range(3):
         again = ops.gemm_fp8_gated(a, a_scale, w, dtype=dtype)
         assert torch.equal(again[0].float(), codes.float()) and torch.equal(again[1], scales)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 72, 200), (5, 1, 100), (5, 72, 200), (200, 300, 1), (5, 72, 128)])
+def test_factory_takes_rows_without_gaps(M, N, K):
+    """As tensors come from elsewhere, the profiler's own among them."""
+    a, a_scale = ops.quant_fp8(randn(M, K, seed=1))
+    w = ops.quant_fp8_weight(randn(N, K, seed=2))
+    kernel = tb.matmul_fp8_block(M, N, K, "float8_e4m3", "float32", "float32")
+    want = ops.gemm_fp8(a, a_scale, w, out_dtype=torch.float32)
+    packed = [t.clone(memory_format=torch.contiguous_format) for t in (a, a_scale, w.codes, w.scales)]
+    assert all(t.is_contiguous() for t in packed)
+    assert torch.equal(kernel(*packed), want) and torch.equal(kernel(a, a_scale, w.codes, w.scales), want)
+    replay, out = kernel.capture(*packed)
+    replay()
+    assert torch.equal(out, want)
+    profiler = kernel.get_profiler()
+    profiler.assert_consistent(repeat=3)
+    assert profiler.do_bench(n_warmup=1, n_repeat=2) > 0
+    tb.check_status()

@@ -541,7 +541,8 @@ def matmul_fp8_block(M: int, N: int, K: int, in_dtype="float8_e4m3", out_dtype="
     """``C[M,N] = A @ B^T`` with both operands in 8-bit floating point: ``kernel(A, A_scale, B, B_scale)`` with A (M, K)
     and one float32 scale for each row and 128 columns (``ops.quant_fp8``), B (N, K) and one for each block of
     128 x 128 (``ops.quant_fp8_weight``). ``in_dtype`` and ``weight_dtype`` (the same unless given) are
-    "float8_e4m3" or "float8_e5m2"; ``out_dtype`` float16, bfloat16 or float32. The weight is read as it is."""
+    "float8_e4m3" or "float8_e5m2"; ``out_dtype`` float16, bfloat16 or float32. The weight is read as it is, unless its
+    rows neither are a multiple of 16 bytes nor lie one apart, as those two functions lay them out: then each call copies it."""
     a_t, out_t = as_torch_dtype(in_dtype), as_torch_dtype(out_dtype)
     w_t = a_t if weight_dtype is None else as_torch_dtype(weight_dtype)
     if a_t not in ops._FP8_OF or w_t not in ops._FP8_OF:
@@ -554,10 +555,14 @@ def matmul_fp8_block(M: int, N: int, K: int, in_dtype="float8_e4m3", out_dtype="
     params = [Param("A", (M, K), a_t), Param("A_scale", (M, kb), torch.float32), Param("B", (N, K), w_t),
               Param("B_scale", (ops._blocks128(N), kb), torch.float32), Param("C", (M, N), out_t)]
 
+    def rows16(t):
+        """Rows without gaps, of a number of bytes that is no multiple of 16, moved apart as the products read them."""
+        return t if K % 16 == 0 or t.shape[0] == 1 or t.stride(0) % 16 == 0 else ops._fp8_rows(*t.shape, t.dtype, t.device).copy_(t)
+
     def impl(kernel: DequantKernel, A, A_scale, B, B_scale):
         for t, p in zip((A, A_scale, B, B_scale), params):
             _check(t, p)
-        return ops.gemm_fp8(A, A_scale, ops.Fp8Weight(B, B_scale), out_dtype=out_t)
+        return ops.gemm_fp8(rows16(A), A_scale, ops.Fp8Weight(rows16(B), B_scale), out_dtype=out_t)
 
     return DequantKernel("matmul_fp8_block", params, [-1], impl, None,
                          f"b200dq kind::f8f6f4 block-scaled: M={M} N={N} K={K} in={a_t} x {w_t} out={out_t}")
