@@ -1,4 +1,8 @@
-"""Sizes that the token exchange refuses still run through ``moe_forward`` over an expert MLP of torch functions."""
+"""Sizes that the token exchange refuses, and calls before the library may be initialised, still run through ``moe_forward`` over an expert MLP of torch functions."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 from torch._subclasses import FakeTensorMode
@@ -44,3 +48,30 @@ def test_wide_rows_and_tokens_without_a_route():
     weights, _ = moe.route(logits, 2)
     # two products of one sign and their sum, a rounding each
     assert torch.allclose(out.double(), x[:6].double() * weights.double().sum(1, keepdim=True), rtol=2 ** -22, atol=0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first", ["", "tb.check_status(); "])
+def test_captured_before_anything_else_has_run(first):
+    """A layer of torch functions as the first call of a process, inside a capture; and as the first after the library's
+    own initialisation."""
+    code = f"""
+import torch
+import tilelang_b200 as tb
+from tilelang_b200 import moe
+{first}
+mlp = moe.ExpertMLP(lambda rows, counts: rows, lambda rows, counts: rows, lambda h: h)
+x, logits = torch.randn(24, 16, device="cuda"), torch.randn(24, 4, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = moe.moe_forward(x, logits, 2, 4, mlp)
+for _ in range(2):
+    x.copy_(torch.randn(24, 16, device="cuda"))
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, moe.moe_forward(x, logits, 2, 4, mlp))
+print("CAPTURED")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, PYTHONPATH=root), cwd=root, capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "CAPTURED" in r.stdout, r.stdout[-2000:] + r.stderr[-3000:]

@@ -383,7 +383,7 @@ def moe_forward(x: torch.Tensor, logits: torch.Tensor, top_k: int, num_experts: 
     weights, experts = route(logits, top_k)
     if isinstance(mlp, Fp8ExpertMLP):
         return mlp.layer(x, experts, weights, num_experts)
-    if (ops._ordinary(x, logits) and x.is_cuda and _fits_exchange(x, logits, top_k, num_experts)
+    if (ops._ordinary(x, logits) and x.is_cuda and _fits_exchange(x, logits, top_k, num_experts) and ops._may_launch(x.device)
             and not (torch.is_grad_enabled() and x.requires_grad)):
         # the same order of rows as below, in one to three launches instead of some ten (torch's gather can be
         # differentiated more than once, forwards, batched and recorded: all of these go on below)

@@ -597,6 +597,11 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # absent
 _current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
+def _may_launch(device: torch.device) -> bool:
+    """Not so where the device would be initialised first, which allocates, while the stream is being captured."""
+    return device.index in _initialised_devices or not torch.cuda.is_current_stream_capturing()
+
+
 def _call(fn, what: str, device: torch.device, *args) -> None:
     """``fn(*args, stream)`` on the device's current stream. Decode steps are a few microseconds on the GPU,
     so the device is switched only when it is not the current one (the context manager and a
